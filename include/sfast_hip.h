@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define SFAST_HIP_ABI_VERSION 9
+#define SFAST_HIP_ABI_VERSION 10
 
 typedef void *sfast_stream_t; /* hipStream_t */
 
@@ -524,6 +524,71 @@ typedef struct {
 } sfast_image_params;
 
 int sfast_hip_image_postprocess(const void *image, void *out, const sfast_image_params *p, sfast_stream_t stream);
+
+/* ---- video attention (ABI 10): positions over several axes, attention over chosen key blocks. Beside sfast_hip_attention; no counterpart
+ * in the reference. ------------------------------------------------------------------------------------------------------------------ */
+
+/* Rotary positions with several axes (time, height, width, ...). Axis a owns sections[a] (even) consecutive elements of every head; pair i of
+ * an axis turns by positions[token][a] * theta^(-2 i / sections[a]) (64-bit angles). Pairs are neighbours (interleaved) or the two halves of
+ * the section. Elements behind the last section are copied. inverse = 1 turns back (the gradient). q: [B, S, H, D], k: [B, S, Hk, D] or NULL
+ * with Hk = 0; strides (b, s, h) in elements, head-dim stride 1; positions [B or 1][S][n_axes], strides (b, s), axis stride 1. */
+#define SFAST_ROPE_MAX_AXES 4
+enum sfast_pos_type { SFAST_POS_I32 = 0, SFAST_POS_I64 = 1, SFAST_POS_F32 = 2, SFAST_POS_F64 = 3 };
+typedef struct {
+    int32_t dtype; /* f16 / bf16 / f32 */
+    int32_t B, S, H, Hk, D; /* D even, <= 256 */
+    int32_t n_axes;
+    int32_t sections[SFAST_ROPE_MAX_AXES];
+    int32_t interleaved, inverse, pos_type;
+    double theta;
+    int64_t qs[3], ks[3], qos[3], kos[3], ps[2];
+} sfast_rope_params;
+int sfast_hip_rope_nd(const void *q, const void *k, const void *positions, void *q_out, void *k_out, const sfast_rope_params *p,
+                      sfast_stream_t stream);
+
+/* Means over blocks of rows: out[b][j][h][:] (fp32, contiguous) = mean of the rows j * block .. of x[b][:][h][:] that lie inside the sequence
+ * (lengths[b], or S when NULL; values outside [0, S] are clipped), summed in 64 bits; a block without rows gives zeros. */
+typedef struct {
+    int32_t dtype; /* f16 / bf16 / f32 */
+    int32_t B, S, H, D, block; /* block: 1 .. 1024 */
+    int64_t xs[3];
+} sfast_block_means_params;
+int sfast_hip_block_means(const void *x, const int32_t *lengths, float *out, const sfast_block_means_params *p, sfast_stream_t stream);
+
+/* Choice of key blocks: out[b][hk][i][:] = the topk blocks j with the largest sum over the group's heads g of qm[b][i][hk * G + g] . km[b][j][hk]
+ * (64 bits), among the blocks that begin inside the sequence (j * block_k < key_lengths[b]). Ascending; ties take the lowest j, a NaN score
+ * ranks above all; -1 behind the last one. qm: [B, nQ, H, D], km: [B, nK, Hk, D] fp32, contiguous, 16-byte aligned, D % 4 == 0, nK <= 32768. */
+typedef struct {
+    int32_t B, nQ, nK, H, Hk, D, topk, block_k;
+} sfast_block_topk_params;
+size_t sfast_hip_block_topk_workspace_bytes(const sfast_block_topk_params *p);
+int sfast_hip_block_topk(const float *qm, const float *km, const int32_t *key_lengths, int32_t *out, const sfast_block_topk_params *p,
+                         void *workspace, size_t workspace_bytes, sfast_stream_t stream);
+
+/* Attention of every query block (block_q = 64 or 128 rows) to the key blocks (block_k = 64 or 128 keys) that blocks[b][hk][query block][:]
+ * names: out = softmax(scale q k^T) v, lse[b][h][s] = log sum exp (natural; fp32). An entry outside [0, ceil(key length / block_k)) names
+ * nothing, an entry named twice counts twice. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key,
+ * give zeros and lse = -inf. Lengths are clipped to [0, S]; NULL: full. q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] (head h reads key head
+ * h / (H / Hk)); strides (b, s, h) in elements, multiples of 8, head-dim stride 1, 16-byte aligned bases; D % 8 == 0, D <= 128. */
+typedef struct {
+    int32_t dtype; /* f16 / bf16 */
+    int32_t B, H, Hk, Sq, Sk, D, block_q, block_k, topk;
+    int64_t qs[3], ks[3], vs[3], os[3];
+    float scale;
+    /* gradients only */
+    int64_t dos[3], dqs[3], dks[3], dvs[3];
+} sfast_block_attn_params;
+size_t sfast_hip_block_attention_workspace_bytes(const sfast_block_attn_params *p);
+int sfast_hip_block_attention(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
+                              const int32_t *query_lengths, void *out, float *lse, const sfast_block_attn_params *p, void *workspace,
+                              size_t workspace_bytes, sfast_stream_t stream);
+/* Gradients of the call above from its out and lse, the gradient dout of out and (or NULL) dlse of lse [B, H, Sq] fp32. All of dq, dk, dv is
+ * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. */
+size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p);
+int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
+                                       const int32_t *query_lengths, const void *out, const float *lse, const void *dout, const float *dlse,
+                                       void *dq, void *dk, void *dv, const sfast_block_attn_params *p, void *workspace, size_t workspace_bytes,
+                                       sfast_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -36,6 +36,8 @@ int igemm_init();      // igemm.hip
 int g_batch_ref = 0;    // common.h
 int attention_init();  // attention.hip
 int gnconv_init();     // gnconv.hip
+int block_attn_init();      // block_attn.hip
+int block_attn_bwd_init();  // block_attn_bwd.hip
 
 }  // namespace sfast
 
@@ -62,6 +64,8 @@ int sfast_hip_init(void) {
         int rc = sfast::igemm_init();
         if (rc == 0) rc = sfast::attention_init();
         if (rc == 0) rc = sfast::gnconv_init();
+        if (rc == 0) rc = sfast::block_attn_init();
+        if (rc == 0) rc = sfast::block_attn_bwd_init();
         state[dev] = rc == 0 ? 1 : rc;
     }
     return state[dev] == 1 ? 0 : state[dev];
