@@ -37,7 +37,9 @@ FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # Per-file additions. attention.hip: the softmax reads every S accumulator and rescales O on the VALU each tile, so MFMA
 # results allocated to AGPRs cost ~150 v_accvgpr moves per 64-key tile (a quarter of the loop); the VGPR form of the MFMA
 # removes them and lowers the register total (D=40: 134+32 -> 138).
-EXTRA_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# block_attn*.hip: the same, every score and dP accumulator is read by the VALU.
+EXTRA_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "block_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+               "block_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # attention_q64.hip (one wave per SIMD, ~400 registers) is built WITHOUT that flag: the O accumulators and the MFMA operand fragments
 # belong in the AGPR half of the unified file, only the S^T tiles the softmax reads must be arch VGPRs.
 

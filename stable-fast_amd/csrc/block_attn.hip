@@ -1,0 +1,372 @@
+// Attention over chosen key blocks, forward (sfast_hip_block_attention).
+//
+// A query block of bq rows attends to the keys of the blocks its list names: o = softmax(scale q k^T) v with a running maximum and sum in
+// fp32, lse = log of the sum. Per row and key 4 D flops on the matrix pipe against ~6 VALU operations for the softmax; K and V of a head are
+// re-read by every query block that names them and live in L2 (each XCD walks a contiguous range of (batch, head, query block)).
+//
+//   * a workgroup is one query block: bq / 32 waves of 32 rows (Q in registers), which stream 64-key K and V tiles through two LDS stages
+//     filled by LDS-DMA (no staging registers); V stays row-major and is read transposed by ds_read_b64_tr_b16.
+//   * few query rows (a token against a long cache): the rows of all heads of a group share a wave (the group shares its list, K and V are
+//     read once), and a list is split over workgroups whose partial results a second launch joins.
+#include "block_attn.h"
+
+namespace sfast {
+
+namespace {
+
+constexpr int BA_MAX_LIST = 1024;  // entries of one workgroup's (part of a) list: 2048 tiles
+
+template <int DP> constexpr int ba_fwd_lds() { return 4 * BaTile<DP>::BYTES + BA_MAX_LIST * 2 * 4 + 16; }
+
+// PACK: rows are (query, head of the group) pairs, row = s * G + g, one unit per key head; else one unit per query head.
+template <typename T, int DP, int NW, bool PACK>
+__global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockAttnArgs a) {
+    using vec8 = typename Elem<T>::vec8;
+    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *tiles = reinterpret_cast<int *>(smem + 4 * TILE);
+    int *ntiles_p = tiles + 2 * BA_MAX_LIST;
+
+    const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
+    // order of the work: (batch, key head, query block, head of the group | part of the list)
+    const int inner = PACK ? a.nsplit : a.G * a.nsplit;
+    const int in = lin % inner, u = lin / inner;
+    const int sp = in % a.nsplit, g0 = PACK ? 0 : in / a.nsplit;
+    const int qb = u % a.nQ, pair = u / a.nQ;
+    const int hk = pair % a.Hk, b = pair / a.Hk;
+    const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
+    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
+
+    const int r = wave * 32 + l31;
+    const int s = PACK ? r / a.G : qb * a.bq + r;
+    const int h = hk * a.G + (PACK ? r - s * a.G : g0);
+    const bool inside = PACK ? s < a.Sq : (r < a.bq && s < a.Sq);  // a row of the output
+    const bool row_ok = inside && s < qlen;
+
+    if (wave == 0) {
+        int n = 0;
+        if ((PACK ? 0 : qb * a.bq) < qlen) {
+            const int e0 = (int)((int64_t)a.topk * sp / a.nsplit), e1 = (int)((int64_t)a.topk * (sp + 1) / a.nsplit);
+            n = ba_tiles(a.blocks + ((int64_t)pair * a.nQ + qb) * a.topk, e0, e1, a.bk, klen, lane, tiles);
+        }
+        if (lane == 0) *ntiles_p = n;
+    }
+
+    // Q: B operand, column = the lane's row
+    const T *Qp = (const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)s * a.qs[1] + (int64_t)h * a.qs[2];
+    vec8 qf[KD];
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+        const int d0 = kd * 16 + hi * 8;
+        u32x4 raw = {0u, 0u, 0u, 0u};
+        if (row_ok && d0 < a.D) raw = *reinterpret_cast<const u32x4 *>(Qp + d0);
+        qf[kd] = __builtin_bit_cast(vec8, raw);
+    }
+
+    const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
+    const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
+    BaLoader<DP, NW> kl, vl;
+    kl.init(wave, lane, a.ks[1], a.D);
+    vl.init(wave, lane, a.vs[1], a.D);
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+    float m = -INFINITY, l = 0.f;  // reference of the row (log2 units) and the lane's share of the sum
+    const float c = a.c;
+
+    __syncthreads();
+    const int n = __builtin_amdgcn_readfirstlane(*ntiles_p);
+    int next = n > 0 ? __builtin_amdgcn_readfirstlane(tiles[0]) : 0;
+    if (n > 0) {
+        kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, smem, wave);
+        vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, smem + TILE, wave);
+    }
+    for (int t = 0; t < n; ++t) {
+        const int cur = next;
+        char *Ks = smem + (t & 1) * (2 * TILE), *Vs = Ks + TILE;
+        if (t + 1 < n) next = __builtin_amdgcn_readfirstlane(tiles[t + 1]);
+        ba_sync();  // tile t has landed, every wave is done with the other stage
+        if (t + 1 < n) {
+            char *Kn = smem + ((t + 1) & 1) * (2 * TILE);
+            kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, Kn, wave);
+            vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, Kn + TILE, wave);
+        }
+        f32x16 sc[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+#pragma unroll
+            for (int kd = 0; kd < KD; ++kd) sc[kb] = ba_mfma(ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi), qf[kd], sc[kb]);
+        }
+        const int left = klen - cur * 64;
+        if (left < 64) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hi >= left) sc[kb][i] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
+        mx = ba_xor32_max(mx) * c;
+        // the reference follows the maximum only when that has grown 256-fold: o / l does not depend on it, and sums and products have the
+        // range for it (f16 probabilities up to 256)
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;  // a row whose scores are all -inf keeps the sum 0
+        vec8 p[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], c, -ref));
+                l += e;
+                p[kb * 2 + (i >> 3)][i & 7] = Elem<T>::from_f32(e);
+            }
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) o[db] = ba_mfma(ba_col_frag<T, DP>(Vs, lane, db, g * 16), p[g], o[db]);
+    }
+    l = ba_xor32_sum(l);
+    if (!inside) return;
+    if (!row_ok) {  // a row behind its sequence: nothing
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+    }
+
+    if (a.nsplit > 1) {
+        const int64_t row = (((int64_t)u * (PACK ? 1 : a.G) + g0) * a.nsplit + sp) * (NW * 32) + r;
+        float *po = a.part_o + row * a.D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = db * 32 + 8 * i + 4 * hi;
+                if (d < a.D) *reinterpret_cast<f32x4 *>(po + d) = f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+            }
+        if (hi == 0) *reinterpret_cast<float2 *>(a.part_ml + row * 2) = make_float2(m, l);
+        return;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no key (or all scores -inf): zeros
+    T *Op = (T *)a.out + (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = db * 32 + 8 * i + 4 * hi;
+            if (d < a.D)
+                *reinterpret_cast<u32x2 *>(Op + d) = pack4<T>(o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv);
+        }
+    if (hi == 0) {
+        float v = -INFINITY;
+        if (!(l == 0.f)) v = (m + __log2f(l)) * 0.69314718055994530942f;
+        a.lse[((int64_t)b * a.H + h) * a.Sq + s] = v;
+    }
+}
+
+// joins the parts of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. One wave a row.
+template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_attn_join_kernel(const BlockAttnArgs a, int rows) {
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);   // (b, hk, qb, g, row of the block) | (b, hk, row)
+    const int per = PACK ? a.Sq * a.G : a.bq;
+    const int64_t unit = id / per;
+    const int r = (int)(id - unit * per);
+    int64_t x = unit;
+    const int g = PACK ? 0 : (int)(x % a.G);
+    if (!PACK) x /= a.G;
+    const int qb = PACK ? 0 : (int)(x % a.nQ);
+    if (!PACK) x /= a.nQ;
+    const int hk = (int)(x % a.Hk), b = (int)(x / a.Hk);
+    if (b >= a.B) return;
+    const int s = PACK ? r / a.G : qb * a.bq + r;
+    const int h = hk * a.G + (PACK ? r - s * a.G : g);
+    if (s >= a.Sq) return;
+    const float *ml = a.part_ml + (unit * a.nsplit * rows + r) * 2;
+    const int64_t step = (int64_t)rows;
+    float M = -INFINITY, L = 0.f;
+    for (int p = lane; p < a.nsplit; p += 64) M = fmaxf(M, ml[p * step * 2]);
+    M = wave_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    for (int p = lane; p < a.nsplit; p += 64) L += __builtin_amdgcn_exp2f(ml[p * step * 2] - ref) * ml[p * step * 2 + 1];
+    L = wave_sum(L);
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const float *po = a.part_o + (unit * a.nsplit * rows + r) * a.D;
+    T *Op = (T *)a.out + (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    for (int d = lane * 2; d < a.D; d += 128) {
+        float x0 = 0.f, x1 = 0.f;
+        for (int p = 0; p < a.nsplit; ++p) {
+            const float w = __builtin_amdgcn_exp2f(ml[p * step * 2] - ref);
+            const float2 v = *reinterpret_cast<const float2 *>(po + p * step * a.D + d);
+            x0 = fmaf(w, v.x, x0);
+            x1 = fmaf(w, v.y, x1);
+        }
+        Op[d] = Elem<T>::from_f32(x0 * inv);
+        Op[d + 1] = Elem<T>::from_f32(x1 * inv);
+    }
+    if (lane == 0) {
+        float v = -INFINITY;
+        if (!(L == 0.f)) v = (M + __log2f(L)) * 0.69314718055994530942f;
+        a.lse[((int64_t)b * a.H + h) * a.Sq + s] = v;
+    }
+}
+
+template <typename T, int DP, int NW, bool PACK> int set_attr() {
+    auto kern = block_attn_fwd_kernel<T, DP, NW, PACK>;
+    const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, ba_fwd_lds<DP>());
+    if (e != hipSuccess) {
+        set_error("hipFuncSetAttribute(block_attn_fwd): %s", hipGetErrorString(e));
+        return SFAST_ERR_LAUNCH;
+    }
+    return 0;
+}
+
+struct Plan {
+    bool pack;
+    int nw, nsplit;
+    int64_t units, nblk;
+};
+
+// How a call is cut into workgroups. Packed rows: all query rows of a group fit 64 rows of one or two waves. A list is split when the
+// query blocks alone would leave compute units empty: 512 workgroups are two on each, and a part keeps at least two tiles.
+static Plan make_plan(const sfast_block_attn_params *p) {
+    Plan pl{};
+    const int G = p->H / p->Hk;
+    const int nQ = ceil_div(p->Sq, p->block_q);
+    pl.pack = nQ == 1 && (int64_t)p->Sq * G <= 64;
+    pl.nw = pl.pack ? (p->Sq * G <= 32 ? 1 : 2) : p->block_q / 32;
+    pl.units = (int64_t)p->B * p->Hk * nQ * (pl.pack ? 1 : G);
+    const int64_t tiles = (int64_t)p->topk * (p->block_k / 64);
+    int64_t ns = 1;
+    if (pl.units < 256) ns = ceil_div64(512, pl.units);
+    if (ns > tiles / 2) ns = tiles / 2;
+    if (ns > p->topk) ns = p->topk;
+    if (ns < 1) ns = 1;
+    const int64_t least = ceil_div64(p->topk, BA_MAX_LIST - 1);  // a part holds at most BA_MAX_LIST entries
+    if (ns < least) ns = least;
+    pl.nsplit = (int)ns;
+    pl.nblk = pl.units * ns;
+    return pl;
+}
+
+template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl, hipStream_t st) {
+    const dim3 grid((unsigned)(8 * a.chunk));
+    const size_t lds = ba_fwd_lds<DP>();
+    if (pl.pack) {
+        if (pl.nw == 1)
+            hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 1, true>), grid, dim3(64), lds, st, a);
+        else
+            hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 2, true>), grid, dim3(128), lds, st, a);
+    } else if (pl.nw == 2) {
+        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 2, false>), grid, dim3(128), lds, st, a);
+    } else {
+        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 4, false>), grid, dim3(256), lds, st, a);
+    }
+    int rc = check_launch("block_attention");
+    if (rc || pl.nsplit == 1) return rc;
+    const int per = pl.pack ? a.Sq * a.G : a.bq;
+    const dim3 jgrid((unsigned)ceil_div64(pl.units * per, 4));
+    if (pl.pack)
+        hipLaunchKernelGGL((block_attn_join_kernel<T, true>), jgrid, dim3(256), 0, st, a, pl.nw * 32);
+    else
+        hipLaunchKernelGGL((block_attn_join_kernel<T, false>), jgrid, dim3(256), 0, st, a, pl.nw * 32);
+    return check_launch("block_attention join");
+}
+
+}  // namespace
+
+int block_attn_check(const sfast_block_attn_params *p) {
+    SFAST_REQUIRE(p, SFAST_ERR_INVALID, "block_attention: null argument");
+    SFAST_REQUIRE(p->dtype == SFAST_F16 || p->dtype == SFAST_BF16, SFAST_ERR_UNSUPPORTED, "block_attention: f16 / bf16 only");
+    SFAST_REQUIRE(p->B > 0 && p->H > 0 && p->Hk > 0 && p->Sq > 0 && p->Sk > 0 && p->D > 0 && p->topk > 0, SFAST_ERR_INVALID, "block_attention: bad shape");
+    SFAST_REQUIRE(p->H % p->Hk == 0, SFAST_ERR_INVALID, "block_attention: %d query heads are no multiple of %d key heads", p->H, p->Hk);
+    SFAST_REQUIRE(p->D % 8 == 0 && p->D <= 128, SFAST_ERR_UNSUPPORTED, "block_attention: head dim %d (a multiple of 8 up to 128 is supported)", p->D);
+    SFAST_REQUIRE((p->block_q == 64 || p->block_q == 128) && (p->block_k == 64 || p->block_k == 128), SFAST_ERR_UNSUPPORTED,
+                  "block_attention: blocks of 64 or 128 rows, got %d / %d", p->block_q, p->block_k);
+    SFAST_REQUIRE(p->scale > 0.f && p->scale < INFINITY, SFAST_ERR_UNSUPPORTED, "block_attention: the scale must be positive and finite");
+    SFAST_REQUIRE(p->Sq <= (1 << 30) && p->Sk <= (1 << 30), SFAST_ERR_UNSUPPORTED, "block_attention: more than 2^30 rows");
+    for (int i = 0; i < 3; ++i)
+        SFAST_REQUIRE(p->qs[i] >= 0 && p->ks[i] >= 0 && p->vs[i] >= 0 && p->qs[i] % 8 == 0 && p->ks[i] % 8 == 0 && p->vs[i] % 8 == 0, SFAST_ERR_UNSUPPORTED,
+                      "block_attention: strides must be multiples of 8 elements");
+    // offsets inside one 64-row tile have 32 bits, bit 31 marks an element outside
+    SFAST_REQUIRE(p->ks[1] < (1 << 23) && p->vs[1] < (1 << 23) && p->qs[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention: row stride too long");
+    return SFAST_OK;
+}
+
+int block_attn_init() {
+    int rc = 0;
+#define SFAST_BA_ATTR(T, DP)                         \
+    if (!rc) rc = set_attr<T, DP, 1, true>();        \
+    if (!rc) rc = set_attr<T, DP, 2, true>();        \
+    if (!rc) rc = set_attr<T, DP, 2, false>();       \
+    if (!rc) rc = set_attr<T, DP, 4, false>();
+    SFAST_BA_ATTR(f16, 64)
+    SFAST_BA_ATTR(f16, 128)
+    SFAST_BA_ATTR(bf16, 64)
+    SFAST_BA_ATTR(bf16, 128)
+#undef SFAST_BA_ATTR
+    return rc;
+}
+
+}  // namespace sfast
+
+using namespace sfast;
+
+extern "C" size_t sfast_hip_block_attention_workspace_bytes(const sfast_block_attn_params *p) {
+    if (block_attn_check(p) != SFAST_OK) return 0;
+    const Plan pl = make_plan(p);
+    if (pl.nsplit == 1) return 0;
+    return (size_t)pl.nblk * (pl.nw * 32) * (p->D + 2) * 4;
+}
+
+extern "C" int sfast_hip_block_attention(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
+                                         const int32_t *query_lengths, void *out, float *lse, const sfast_block_attn_params *p, void *workspace,
+                                         size_t workspace_bytes, sfast_stream_t stream) {
+    SFAST_REQUIRE(q && k && v && blocks && out && lse, SFAST_ERR_INVALID, "block_attention: null argument");
+    int rc = block_attn_check(p);
+    if (rc != SFAST_OK) return rc;
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
+    for (int i = 0; i < 3; ++i) SFAST_REQUIRE(p->os[i] % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_attention: output strides must be multiples of 4 elements");
+    const Plan pl = make_plan(p);
+    SFAST_REQUIRE(pl.nblk <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
+    BlockAttnArgs a{};
+    a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.lse = lse;
+    a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
+    a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
+    for (int i = 0; i < 3; ++i) a.qs[i] = p->qs[i], a.ks[i] = p->ks[i], a.vs[i] = p->vs[i], a.os[i] = p->os[i];
+    a.scale = p->scale;
+    a.c = p->scale * 1.44269504088896340736f;
+    a.nsplit = pl.nsplit;
+    a.nblk = (int)pl.nblk;
+    a.chunk = (int)ceil_div64(pl.nblk, 8);
+    if (pl.nsplit > 1) {
+        SFAST_REQUIRE(workspace && workspace_bytes >= sfast_hip_block_attention_workspace_bytes(p) && aligned16(workspace), SFAST_ERR_WORKSPACE,
+                      "block_attention: workspace too small");
+        a.part_o = (float *)workspace;
+        a.part_ml = a.part_o + (size_t)pl.nblk * (pl.nw * 32) * p->D;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    set_kernel_name("block_attn_fwd[DP=%d,rows=%d,split=%d%s]", p->D <= 64 ? 64 : 128, pl.nw * 32, pl.nsplit, pl.pack ? ",packed" : "");
+    if (p->dtype == SFAST_F16) return p->D <= 64 ? launch<f16, 64>(a, pl, st) : launch<f16, 128>(a, pl, st);
+    return p->D <= 64 ? launch<bf16, 64>(a, pl, st) : launch<bf16, 128>(a, pl, st);
+}

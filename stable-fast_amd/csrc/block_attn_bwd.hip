@@ -1,0 +1,429 @@
+// Attention over chosen key blocks, gradients (sfast_hip_block_attention_backward).
+//
+// With P = exp(s - lse): dV = P^T dO, dP = dO V^T, dS = P (dP - delta), dQ = scale dS K, dK = scale dS^T Q, delta = rowsum(dO O) - dlse.
+// Bound by the matrix pipe (seven products a tile pair: the scores and dP are made twice) together with the LDS operand reads.
+//
+//   * two kernels instead of atomics, so that the same call gives the same bits: one streams the listed key blocks past a query block (dQ),
+//     one streams the query blocks past a key block (dK, dV).
+//   * the second needs the lists the other way round: a small kernel counts, per key block, how often each query block names it (integer
+//     atomics: their order changes nothing), and the workgroup of a key block walks its row of counts. A count m enters as
+//     2^(s - lse + log2 m).
+//   * both keep their own rows' operands and sums in registers and read the streamed tiles from LDS as rows (scores, dP) and transposed (sums).
+#include "block_attn.h"
+
+namespace sfast {
+
+namespace {
+
+constexpr int BB_LIST = 1024;  // list entries held in LDS at a time
+constexpr float LOG2E = 1.44269504088896340736f;
+
+template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 16; }
+template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 2 * 2 * 64 * 4 + 16; }
+
+// delta of a row: 16 lanes, 8 elements each
+template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, s, h)
+    const int d = (threadIdx.x & 15) * 8;
+    if (row >= (int64_t)a.B * a.Sq * a.H) return;
+    const int h = (int)(row % a.H);
+    const int64_t bs = row / a.H;
+    const int s = (int)(bs % a.Sq), b = (int)(bs / a.Sq);
+    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
+    float sum = 0.f;
+    if (s < qlen && d < a.D) {
+        float x[8], y[8];
+        unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.dout + b * a.dos[0] + s * a.dos[1] + h * a.dos[2] + d), x);
+        unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.o + b * a.os[0] + s * a.os[1] + h * a.os[2] + d), y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
+    }
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (d == 0) {
+        const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
+        if (a.dlse && s < qlen) sum -= a.dlse[at];
+        a.delta[at] = sum;
+    }
+}
+
+__global__ void __launch_bounds__(256) block_attn_zero_kernel(int32_t *p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+
+// cnt[pair][key block][query block] += 1 for every entry that names something
+__global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnArgs a, int64_t entries) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= entries) return;
+    const int64_t list = e / a.topk, pair = list / a.nQ;
+    const int qb = (int)(list - pair * a.nQ), b = (int)(pair / a.Hk);
+    const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
+    const int j = a.blocks[e];
+    if (j >= 0 && (int64_t)j * a.bk < klen) atomicAdd(a.cnt + (pair * a.nK + j) * a.nQ + qb, 1);
+}
+
+// dQ of one query block: the forward's streams, K read as rows (scores) and transposed (dQ), V as rows (dP)
+template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
+    using vec8 = typename Elem<T>::vec8;
+    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *tiles = reinterpret_cast<int *>(smem + 4 * TILE);
+    int *ntiles_p = tiles + 2 * BB_LIST;
+
+    const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
+    const int g0 = lin % a.G, u = lin / a.G;
+    const int qb = u % a.nQ, pair = u / a.nQ;
+    const int hk = pair % a.Hk, b = pair / a.Hk, h = hk * a.G + g0;
+    const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
+    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
+    const int s = qb * a.bq + wave * 32 + l31;
+    const bool row_ok = s < qlen;
+
+    const T *Qp = (const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)s * a.qs[1] + (int64_t)h * a.qs[2];
+    const T *Gp = (const T *)a.dout + (int64_t)b * a.dos[0] + (int64_t)s * a.dos[1] + (int64_t)h * a.dos[2];
+    vec8 qf[KD], gf[KD];
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+        const int d0 = kd * 16 + hi * 8;
+        u32x4 x = {0u, 0u, 0u, 0u}, y = {0u, 0u, 0u, 0u};
+        if (row_ok && d0 < a.D) {
+            x = *reinterpret_cast<const u32x4 *>(Qp + d0);
+            y = *reinterpret_cast<const u32x4 *>(Gp + d0);
+        }
+        qf[kd] = __builtin_bit_cast(vec8, x);
+        gf[kd] = __builtin_bit_cast(vec8, y);
+    }
+    float L = INFINITY, delta = 0.f;  // a row without keys: probabilities 0
+    if (row_ok) {
+        const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
+        const float v = a.lse[at];
+        if (v != -INFINITY) L = v * LOG2E;
+        delta = a.delta[at];
+    }
+    const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
+    const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
+    BaLoader<DP, NW> kl, vl;
+    kl.init(wave, lane, a.ks[1], a.D);
+    vl.init(wave, lane, a.vs[1], a.D);
+    f32x16 dq[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
+    const float c = a.c;
+
+    const int e_all = qb * a.bq < qlen ? a.topk : 0;
+    for (int e0 = 0; e0 < e_all; e0 += BB_LIST) {
+        __syncthreads();
+        if (wave == 0) {
+            const int n = ba_tiles(a.blocks + ((int64_t)pair * a.nQ + qb) * a.topk, e0, min(e0 + BB_LIST, e_all), a.bk, klen, lane, tiles);
+            if (lane == 0) *ntiles_p = n;
+        }
+        __syncthreads();
+        const int n = __builtin_amdgcn_readfirstlane(*ntiles_p);
+        int next = n > 0 ? __builtin_amdgcn_readfirstlane(tiles[0]) : 0;
+        if (n > 0) {
+            kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, smem, wave);
+            vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, smem + TILE, wave);
+        }
+        for (int t = 0; t < n; ++t) {
+            const int cur = next;
+            char *Ks = smem + (t & 1) * (2 * TILE), *Vs = Ks + TILE;
+            if (t + 1 < n) next = __builtin_amdgcn_readfirstlane(tiles[t + 1]);
+            ba_sync();
+            if (t + 1 < n) {
+                char *Kn = smem + ((t + 1) & 1) * (2 * TILE);
+                kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, Kn, wave);
+                vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, Kn + TILE, wave);
+            }
+            const int left = klen - cur * 64;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                f32x16 sc, dp;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) sc = ba_mfma(ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi), qf[kd], sc);
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) dp = ba_mfma(ba_row_frag<T, DP>(Vs, kb * 32 + l31, kd, hi), gf[kd], dp);
+                if (left < 64) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hi >= left) sc[i] = -INFINITY;
+                }
+                vec8 ds[2];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L));
+                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * (dp[i] - delta));
+                }
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) dq[db] = ba_mfma(ba_col_frag<T, DP>(Ks, lane, db, kb * 32 + g * 16), ds[g], dq[db]);
+            }
+        }
+    }
+    if (s >= a.Sq) return;
+    T *Op = (T *)a.dq + (int64_t)b * a.dqs[0] + (int64_t)s * a.dqs[1] + (int64_t)h * a.dqs[2];
+    const float k = row_ok ? a.scale : 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = db * 32 + 8 * i + 4 * hi;
+            if (d < a.D)
+                *reinterpret_cast<u32x2 *>(Op + d) = pack4<T>(dq[db][4 * i] * k, dq[db][4 * i + 1] * k, dq[db][4 * i + 2] * k, dq[db][4 * i + 3] * k);
+        }
+}
+
+// dK and dV of one key block: NW waves of 32 keys (K and V in registers as the lanes' columns), streaming 64-row tiles of Q and dO of the query
+// blocks that name it, of all heads of the group
+template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dkv_kernel(const BlockAttnArgs a) {
+    using vec8 = typename Elem<T>::vec8;
+    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, NT = NW * 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int *names = reinterpret_cast<int *>(smem + 4 * TILE);       // query block, count of it
+    float *stat = reinterpret_cast<float *>(names + 2 * BB_LIST);  // two stages of 64 (lse in log2 units - log2 count), 64 delta
+    int *n_p = reinterpret_cast<int *>(stat + 2 * 2 * 64);
+
+    const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
+    const int j = lin % a.nK, pair = lin / a.nK;
+    const int hk = pair % a.Hk, b = pair / a.Hk;
+    const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
+    const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
+    const int64_t key = (int64_t)j * a.bk + wave * 32 + l31;
+    const bool key_ok = key < klen;
+
+    const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + key * a.ks[1] + (int64_t)hk * a.ks[2];
+    const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + key * a.vs[1] + (int64_t)hk * a.vs[2];
+    vec8 kf[KD], vf[KD];
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+        const int d0 = kd * 16 + hi * 8;
+        u32x4 x = {0u, 0u, 0u, 0u}, y = {0u, 0u, 0u, 0u};
+        if (key_ok && d0 < a.D) {
+            x = *reinterpret_cast<const u32x4 *>(Kp + d0);
+            y = *reinterpret_cast<const u32x4 *>(Vp + d0);
+        }
+        kf[kd] = __builtin_bit_cast(vec8, x);
+        vf[kd] = __builtin_bit_cast(vec8, y);
+    }
+    BaLoader<DP, NW> ql, gl;
+    ql.init(wave, lane, a.qs[1], a.D);
+    gl.init(wave, lane, a.dos[1], a.D);
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[db][i] = 0.f, dv[db][i] = 0.f;
+    const float c = a.c;
+    const int subs = a.bq >> 6, per = a.G * subs;
+    const int32_t *cnt = a.cnt + ((int64_t)pair * a.nK + j) * a.nQ;
+
+    // step x of a list: entry x / per, head (x % per) / subs, 64-row tile x % subs of the query block
+    const auto request = [&](int x, int stage) __attribute__((always_inline)) {
+        const int e = x / per, y = x - e * per, g = y / subs, sub = y - g * subs;
+        const int qb = __builtin_amdgcn_readfirstlane(names[2 * e]);
+        const int h = hk * a.G + g, s0 = qb * a.bq + sub * 64;
+        char *Qs = smem + stage * (2 * TILE);
+        ql.load((const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)h * a.qs[2], a.qs[1], a.D, s0, qlen - s0, Qs, wave);
+        gl.load((const T *)a.dout + (int64_t)b * a.dos[0] + (int64_t)h * a.dos[2], a.dos[1], a.D, s0, qlen - s0, Qs + TILE, wave);
+        if (tid < 64) {
+            float L = INFINITY, dl = 0.f;
+            if (s0 + tid < qlen) {
+                const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s0 + tid;
+                const float v = a.lse[at];
+                if (v != -INFINITY) L = v * LOG2E - __log2f((float)names[2 * e + 1]);
+                dl = a.delta[at];
+            }
+            stat[stage * 128 + tid] = L;
+            stat[stage * 128 + 64 + tid] = dl;
+        }
+    };
+
+    const int i_all = (int64_t)j * a.bk < klen ? (qlen + a.bq - 1) / a.bq : 0;
+    for (int i0 = 0; i0 < i_all; i0 += BB_LIST) {
+        __syncthreads();
+        if (wave == 0) {
+            int n = 0;
+            for (int i = i0; i < min(i0 + BB_LIST, i_all); i += 64) {
+                const int m = i + lane < min(i0 + BB_LIST, i_all) ? cnt[i + lane] : 0;
+                const uint64_t some = __ballot(m > 0);
+                const int at = n + __popcll(some & ((1ull << lane) - 1));
+                if (m > 0) names[2 * at] = i + lane, names[2 * at + 1] = m;
+                n += __popcll(some);
+            }
+            if (lane == 0) *n_p = n;
+        }
+        __syncthreads();
+        const int steps = __builtin_amdgcn_readfirstlane(*n_p) * per;
+        if (steps > 0) request(0, 0);
+        for (int x = 0; x < steps; ++x) {
+            const char *Qs = smem + (x & 1) * (2 * TILE), *Gs = Qs + TILE;
+            const float *Ls = stat + (x & 1) * 128;
+            ba_sync();
+            if (x + 1 < steps) request(x + 1, (x + 1) & 1);
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                f32x16 sc, dp;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) sc = ba_mfma(ba_row_frag<T, DP>(Qs, rb * 32 + l31, kd, hi), kf[kd], sc);
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) dp = ba_mfma(ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi), vf[kd], dp);
+                vec8 p8[2], ds[2];
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    const f32x4 L = *reinterpret_cast<const f32x4 *>(Ls + rb * 32 + 8 * q4 + 4 * hi);
+                    const f32x4 dl = *reinterpret_cast<const f32x4 *>(Ls + 64 + rb * 32 + 8 * q4 + 4 * hi);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 4 * q4 + r;
+                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L[r]));
+                        p8[i >> 3][i & 7] = Elem<T>::from_f32(p);
+                        ds[i >> 3][i & 7] = Elem<T>::from_f32(p * (dp[i] - dl[r]));
+                    }
+                }
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        dv[db] = ba_mfma(ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16), p8[g], dv[db]);
+                        dk[db] = ba_mfma(ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16), ds[g], dk[db]);
+                    }
+            }
+        }
+    }
+    if (key >= a.Sk) return;
+    T *Kg = (T *)a.dk + (int64_t)b * a.dks[0] + key * a.dks[1] + (int64_t)hk * a.dks[2];
+    T *Vg = (T *)a.dv + (int64_t)b * a.dvs[0] + key * a.dvs[1] + (int64_t)hk * a.dvs[2];
+    const float k = a.scale;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = db * 32 + 8 * i + 4 * hi;
+            if (d < a.D) {
+                u32x2 x = pack4<T>(dk[db][4 * i] * k, dk[db][4 * i + 1] * k, dk[db][4 * i + 2] * k, dk[db][4 * i + 3] * k);
+                u32x2 y = pack4<T>(dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]);
+                if (!key_ok) x = u32x2{0u, 0u}, y = u32x2{0u, 0u};  // a key behind the sequence
+                *reinterpret_cast<u32x2 *>(Kg + d) = x;
+                *reinterpret_cast<u32x2 *>(Vg + d) = y;
+            }
+        }
+}
+
+template <typename T, int DP> int set_attr() {
+    hipError_t e = hipSuccess;
+    const auto one = [&](const void *kern, int bytes) {
+        if (e == hipSuccess) e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    one((const void *)block_attn_dq_kernel<T, DP, 2>, bb_dq_lds<DP>());
+    one((const void *)block_attn_dq_kernel<T, DP, 4>, bb_dq_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 2>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 4>, bb_dkv_lds<DP>());
+    if (e != hipSuccess) {
+        set_error("hipFuncSetAttribute(block_attn_bwd): %s", hipGetErrorString(e));
+        return SFAST_ERR_LAUNCH;
+    }
+    return 0;
+}
+
+template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
+    const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ, entries = (int64_t)a.B * a.Hk * a.nQ * a.topk;
+    const int64_t rows = (int64_t)a.B * a.Sq * a.H;
+    hipLaunchKernelGGL(block_attn_zero_kernel, dim3((unsigned)(cells < 1024 * 256 ? ceil_div64(cells, 256) : 1024)), dim3(256), 0, st, a.cnt, cells);
+    int rc = check_launch("block_attention_backward zero");
+    if (rc) return rc;
+    hipLaunchKernelGGL(block_attn_count_kernel, dim3((unsigned)ceil_div64(entries, 256)), dim3(256), 0, st, a, entries);
+    rc = check_launch("block_attention_backward count");
+    if (rc) return rc;
+    hipLaunchKernelGGL((block_attn_delta_kernel<T>), dim3((unsigned)ceil_div64(rows, 16)), dim3(256), 0, st, a);
+    rc = check_launch("block_attention_backward delta");
+    if (rc) return rc;
+    a.nblk = a.B * a.Hk * a.nQ * a.G;
+    a.chunk = ceil_div(a.nblk, 8);
+    if (a.bq == 64)
+        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 2>), dim3(8 * a.chunk), dim3(128), bb_dq_lds<DP>(), st, a);
+    else
+        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 4>), dim3(8 * a.chunk), dim3(256), bb_dq_lds<DP>(), st, a);
+    rc = check_launch("block_attention_backward dq");
+    if (rc) return rc;
+    a.nblk = a.B * a.Hk * a.nK;
+    a.chunk = ceil_div(a.nblk, 8);
+    if (a.bk == 64)
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2>), dim3(8 * a.chunk), dim3(128), bb_dkv_lds<DP>(), st, a);
+    else
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
+    return check_launch("block_attention_backward dkv");
+}
+
+static int64_t delta_floats(const sfast_block_attn_params *p) { return ((int64_t)p->B * p->H * p->Sq + 3) / 4 * 4; }
+static int64_t cells(const sfast_block_attn_params *p) {
+    return (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) * ceil_div(p->Sq, p->block_q);
+}
+
+}  // namespace
+
+int block_attn_bwd_init() {
+    int rc = set_attr<f16, 64>();
+    if (!rc) rc = set_attr<f16, 128>();
+    if (!rc) rc = set_attr<bf16, 64>();
+    if (!rc) rc = set_attr<bf16, 128>();
+    return rc;
+}
+
+}  // namespace sfast
+
+using namespace sfast;
+
+extern "C" size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p) {
+    if (block_attn_check(p) != SFAST_OK) return 0;
+    return (size_t)(delta_floats(p) + cells(p)) * 4;
+}
+
+extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
+                                                  const int32_t *query_lengths, const void *out, const float *lse, const void *dout, const float *dlse,
+                                                  void *dq, void *dk, void *dv, const sfast_block_attn_params *p, void *workspace,
+                                                  size_t workspace_bytes, sfast_stream_t stream) {
+    SFAST_REQUIRE(q && k && v && blocks && out && lse && dout && dq && dk && dv, SFAST_ERR_INVALID, "block_attention_backward: null argument");
+    int rc = block_attn_check(p);
+    if (rc != SFAST_OK) return rc;
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned8(dq) && aligned8(dk) && aligned8(dv),
+                  SFAST_ERR_UNSUPPORTED, "block_attention_backward: operands must be 16-byte aligned");
+    for (int i = 0; i < 3; ++i) {
+        SFAST_REQUIRE(p->os[i] % 8 == 0 && p->dos[i] % 8 == 0 && p->os[i] >= 0 && p->dos[i] >= 0, SFAST_ERR_UNSUPPORTED,
+                      "block_attention_backward: strides must be multiples of 8 elements");
+        SFAST_REQUIRE(p->dqs[i] % 4 == 0 && p->dks[i] % 4 == 0 && p->dvs[i] % 4 == 0, SFAST_ERR_UNSUPPORTED,
+                      "block_attention_backward: gradient strides must be multiples of 4 elements");
+    }
+    SFAST_REQUIRE(p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: row stride too long");
+    SFAST_REQUIRE((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) <= (1ll << 30) && (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) <= (1ll << 30) &&
+                      (int64_t)p->B * p->Sq * p->H <= (1ll << 34) && (int64_t)p->B * p->Hk * ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 38),
+                  SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
+    SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
+                  "block_attention_backward: workspace too small");
+    BlockAttnArgs a{};
+    a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float *>(lse), a.dlse = dlse, a.dq = dq, a.dk = dk, a.dv = dv;
+    a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths;
+    a.delta = (float *)workspace;
+    a.cnt = (int32_t *)(a.delta + delta_floats(p));
+    a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
+    a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = p->qs[i], a.ks[i] = p->ks[i], a.vs[i] = p->vs[i], a.os[i] = p->os[i], a.dos[i] = p->dos[i];
+        a.dqs[i] = p->dqs[i], a.dks[i] = p->dks[i], a.dvs[i] = p->dvs[i];
+    }
+    a.scale = p->scale;
+    a.c = p->scale * LOG2E;
+    hipStream_t st = (hipStream_t)stream;
+    set_kernel_name("block_attn_bwd[DP=%d]", p->D <= 64 ? 64 : 128);
+    if (p->dtype == SFAST_F16) return p->D <= 64 ? launch<f16, 64>(a, st) : launch<f16, 128>(a, st);
+    return p->D <= 64 ? launch<bf16, 64>(a, st) : launch<bf16, 128>(a, st);
+}

@@ -10,3 +10,4 @@ __version__ = "0.1.0+mi355x"
 from . import torch_ops  # noqa: F401,E402  (torch.ops.sfast.*)
 from .triton import torch_ops as _triton_ops  # noqa: F401,E402  (torch.ops.sfast_triton.*)
 from .libs.xformers import xformers_attention as _xf_ops  # noqa: F401,E402  (torch.ops.sfast_xformers.*)
+from .libs.xformers import sparse_attention as _sparse_ops  # noqa: F401,E402  (block means / choice / attention)

@@ -18,7 +18,7 @@ PROBES_LIB_PATH = os.path.join(os.path.dirname(_HERE), "_lib", "libsfast_hip_pro
 if os.environ.get("SFAST_HIP_PROBES", "0") == "1":
     LIB_PATH = PROBES_LIB_PATH
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 # enums (include/sfast_hip.h)
 F16, BF16, F32 = 0, 1, 2
@@ -41,7 +41,12 @@ EXPORTS = [
     "sfast_hip_schedule_advance", "sfast_hip_conv2d_plan", "sfast_hip_workspace_init", "sfast_hip_has_probes",
     "sfast_hip_gn_conv2d_supported", "sfast_hip_gn_conv2d_workspace_bytes", "sfast_hip_gn_conv2d",
     "sfast_hip_lora_merge_plan", "sfast_hip_lora_merge", "sfast_hip_packed_weight_bytes", "sfast_hip_pack_weight",
+    "sfast_hip_rope_nd", "sfast_hip_block_means", "sfast_hip_block_topk_workspace_bytes", "sfast_hip_block_topk",
+    "sfast_hip_block_attention_workspace_bytes", "sfast_hip_block_attention",
+    "sfast_hip_block_attention_backward_workspace_bytes", "sfast_hip_block_attention_backward",
 ]
+ROPE_MAX_AXES = 4
+POS_I32, POS_I64, POS_F32, POS_F64 = range(4)
 LORA_MAX_RANK = 128
 
 
@@ -148,6 +153,30 @@ class TembParams(C.Structure):
                 ("max_period", C.c_float)]
 
 
+class RopeParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("S", C.c_int32), ("H", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
+                ("n_axes", C.c_int32), ("sections", C.c_int32 * ROPE_MAX_AXES), ("interleaved", C.c_int32), ("inverse", C.c_int32),
+                ("pos_type", C.c_int32), ("theta", C.c_double), ("qs", C.c_int64 * 3), ("ks", C.c_int64 * 3), ("qos", C.c_int64 * 3),
+                ("kos", C.c_int64 * 3), ("ps", C.c_int64 * 2)]
+
+
+class BlockMeansParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("S", C.c_int32), ("H", C.c_int32), ("D", C.c_int32), ("block", C.c_int32),
+                ("xs", C.c_int64 * 3)]
+
+
+class BlockTopkParams(C.Structure):
+    _fields_ = [("B", C.c_int32), ("nQ", C.c_int32), ("nK", C.c_int32), ("H", C.c_int32), ("Hk", C.c_int32), ("D", C.c_int32),
+                ("topk", C.c_int32), ("block_k", C.c_int32)]
+
+
+class BlockAttnParams(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("Hk", C.c_int32), ("Sq", C.c_int32), ("Sk", C.c_int32),
+                ("D", C.c_int32), ("block_q", C.c_int32), ("block_k", C.c_int32), ("topk", C.c_int32),
+                ("qs", C.c_int64 * 3), ("ks", C.c_int64 * 3), ("vs", C.c_int64 * 3), ("os", C.c_int64 * 3), ("scale", C.c_float),
+                ("dos", C.c_int64 * 3), ("dqs", C.c_int64 * 3), ("dks", C.c_int64 * 3), ("dvs", C.c_int64 * 3)]
+
+
 class SfastHipError(RuntimeError):
     pass
 
@@ -236,6 +265,22 @@ def _declare(lib):
     lib.sfast_hip_gn_conv2d_workspace_bytes.argtypes = [C.POINTER(GnConvParams)]
     lib.sfast_hip_gn_conv2d.restype = C.c_int
     lib.sfast_hip_gn_conv2d.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, C.POINTER(GnConvParams), vp, sz, vp]
+    lib.sfast_hip_rope_nd.restype = C.c_int
+    lib.sfast_hip_rope_nd.argtypes = [vp, vp, vp, vp, vp, C.POINTER(RopeParams), vp]
+    lib.sfast_hip_block_means.restype = C.c_int
+    lib.sfast_hip_block_means.argtypes = [vp, vp, vp, C.POINTER(BlockMeansParams), vp]
+    lib.sfast_hip_block_topk_workspace_bytes.restype = sz
+    lib.sfast_hip_block_topk_workspace_bytes.argtypes = [C.POINTER(BlockTopkParams)]
+    lib.sfast_hip_block_topk.restype = C.c_int
+    lib.sfast_hip_block_topk.argtypes = [vp, vp, vp, vp, C.POINTER(BlockTopkParams), vp, sz, vp]
+    lib.sfast_hip_block_attention_workspace_bytes.restype = sz
+    lib.sfast_hip_block_attention_workspace_bytes.argtypes = [C.POINTER(BlockAttnParams)]
+    lib.sfast_hip_block_attention.restype = C.c_int
+    lib.sfast_hip_block_attention.argtypes = [vp] * 8 + [C.POINTER(BlockAttnParams), vp, sz, vp]
+    lib.sfast_hip_block_attention_backward_workspace_bytes.restype = sz
+    lib.sfast_hip_block_attention_backward_workspace_bytes.argtypes = [C.POINTER(BlockAttnParams)]
+    lib.sfast_hip_block_attention_backward.restype = C.c_int
+    lib.sfast_hip_block_attention_backward.argtypes = [vp] * 13 + [C.POINTER(BlockAttnParams), vp, sz, vp]
     lib.sfast_hip_cfg_ddim_step.restype = C.c_int
     lib.sfast_hip_cfg_ddim_step.argtypes = [vp, vp, vp, vp, vp, C.c_float, C.c_int64, C.c_int32, vp]
 
