@@ -5,6 +5,7 @@
 
 Every csrc/*.hip is compiled to an object (in parallel) and linked into
 stable-fast_amd/sfast/_lib/libsfast_hip.so. hipcc cross-compiles without a GPU.
+csrc/torch/*.cpp (native torch operators on the C ABI, host code) becomes sfast/_lib/libsfast_torch.so beside it.
 Objects are cached by (source + headers + flags) hash so rebuilds are incremental.
 
 --probes builds a SECOND library, sfast/_lib/libsfast_hip_probes.so, with -DSFAST_PROBES: the timing-only experiment / ablation
@@ -27,6 +28,8 @@ OUT_DIR = os.path.join(HERE, "sfast", "_lib")
 OBJ_DIR = os.path.join(HERE, "build", "obj")
 LIB = os.path.join(OUT_DIR, "libsfast_hip.so")
 LIB_PROBES = os.path.join(OUT_DIR, "libsfast_hip_probes.so")
+CSRC_TORCH = os.path.join(CSRC, "torch")
+LIB_TORCH = os.path.join(OUT_DIR, "libsfast_torch.so")
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast",
          "-Wno-unused-result", "-I", INCLUDE]
@@ -58,6 +61,33 @@ def _digest(paths, extra):
             h.update(f.read())
     h.update(" ".join(extra).encode())
     return h.hexdigest()[:16]
+
+
+def build_torch_ops(force=False, verbose=True):
+    """csrc/torch/*.cpp: native torch operators on the C ABI -> sfast/_lib/libsfast_torch.so (host code; finds libsfast_hip.so beside itself,
+    torch's own libraries are in the process already)."""
+    import importlib.util
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)   # (not imported: its headers and libraries are enough)
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        version = f.read()
+    srcs = sorted(os.path.join(CSRC_TORCH, f) for f in os.listdir(CSRC_TORCH) if f.endswith(".cpp"))
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-isystem", os.path.join(torch_dir, "include"),
+             "-isystem", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), "-isystem", os.path.join(os.path.dirname(os.path.dirname(hipcc())), "include")]
+    tag = _digest(srcs + [os.path.join(INCLUDE, "sfast_hip.h")], flags + [version])
+    stamp = os.path.join(OBJ_DIR, "torch_ops.stamp")
+    if not force and os.path.exists(LIB_TORCH) and os.path.exists(stamp) and open(stamp).read() == tag:
+        return LIB_TORCH
+    lib = os.path.join(torch_dir, "lib")
+    cmd = [shutil.which("g++") or "g++"] + flags + ["-shared", "-o", LIB_TORCH] + srcs + ["-L" + OUT_DIR, "-lsfast_hip", "-Wl,-rpath,$ORIGIN", "-L" + lib,
+                                                                                            "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for csrc/torch:\n{r.stderr[-4000:]}")
+    with open(stamp, "w") as f:
+        f.write(tag)
+    if verbose:
+        print(f"[sfast build] linked {LIB_TORCH}", flush=True)
+    return LIB_TORCH
 
 
 def build(force=False, jobs=None, verbose=True, probes=False):
@@ -110,6 +140,8 @@ def build(force=False, jobs=None, verbose=True, probes=False):
         p = os.path.join(OBJ_DIR, f)
         if f.endswith(".o") and p not in keep and ((".p." in f) == probes):
             os.remove(p)
+    if not probes:
+        build_torch_ops(force, verbose)
     return lib_path
 
 

@@ -13,8 +13,8 @@
 namespace sfast {
 
 struct BlockAttnArgs {
-    const void *q, *k, *v, *dout, *o;
-    void *out, *dq, *dk, *dv;
+    const void *q, *k, *v, *dout, *o, *o_rest;
+    void *out, *out_rest, *dq, *dk, *dv;  // out_rest: what the rounding of out left, or NULL
     float *lse;                // [B, H, Sq], natural log
     const float *dlse;         // gradient of lse, or NULL
     float *delta;              // [B, H, Sq]: rowsum(dout * o) - dlse

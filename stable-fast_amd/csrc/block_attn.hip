@@ -169,14 +169,23 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
         return;
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no key (or all scores -inf): zeros
-    T *Op = (T *)a.out + (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    const int64_t at = (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    T *Op = (T *)a.out + at;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = db * 32 + 8 * i + 4 * hi;
-            if (d < a.D)
-                *reinterpret_cast<u32x2 *>(Op + d) = pack4<T>(o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv);
+            if (d < a.D) {
+                const float x[4] = {o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv};
+                const u32x2 y = pack4<T>(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<u32x2 *>(Op + d) = y;
+                if (a.out_rest) {
+                    float z[4];
+                    unpack4<T>(y, z);
+                    *reinterpret_cast<u32x2 *>((T *)a.out_rest + at + d) = pack4<T>(x[0] - z[0], x[1] - z[1], x[2] - z[2], x[3] - z[3]);
+                }
+            }
         }
     if (hi == 0) {
         float v = -INFINITY;
@@ -212,7 +221,8 @@ template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_at
     L = wave_sum(L);
     const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
     const float *po = a.part_o + (unit * a.nsplit * rows + r) * a.D;
-    T *Op = (T *)a.out + (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    const int64_t at = (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    T *Op = (T *)a.out + at;
     for (int d = lane * 2; d < a.D; d += 128) {
         float x0 = 0.f, x1 = 0.f;
         for (int p = 0; p < a.nsplit; ++p) {
@@ -221,8 +231,13 @@ template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_at
             x0 = fmaf(w, v.x, x0);
             x1 = fmaf(w, v.y, x1);
         }
-        Op[d] = Elem<T>::from_f32(x0 * inv);
-        Op[d + 1] = Elem<T>::from_f32(x1 * inv);
+        const T y0 = Elem<T>::from_f32(x0 * inv), y1 = Elem<T>::from_f32(x1 * inv);
+        Op[d] = y0;
+        Op[d + 1] = y1;
+        if (a.out_rest) {
+            ((T *)a.out_rest)[at + d] = Elem<T>::from_f32(x0 * inv - (float)y0);
+            ((T *)a.out_rest)[at + d + 1] = Elem<T>::from_f32(x1 * inv - (float)y1);
+        }
     }
     if (lane == 0) {
         float v = -INFINITY;
@@ -340,17 +355,17 @@ extern "C" size_t sfast_hip_block_attention_workspace_bytes(const sfast_block_at
 }
 
 extern "C" int sfast_hip_block_attention(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
-                                         const int32_t *query_lengths, void *out, float *lse, const sfast_block_attn_params *p, void *workspace,
-                                         size_t workspace_bytes, sfast_stream_t stream) {
+                                         const int32_t *query_lengths, void *out, float *lse, void *out_rest, const sfast_block_attn_params *p,
+                                         void *workspace, size_t workspace_bytes, sfast_stream_t stream) {
     SFAST_REQUIRE(q && k && v && blocks && out && lse, SFAST_ERR_INVALID, "block_attention: null argument");
     int rc = block_attn_check(p);
     if (rc != SFAST_OK) return rc;
-    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out) && aligned8(out_rest), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) SFAST_REQUIRE(p->os[i] % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_attention: output strides must be multiples of 4 elements");
     const Plan pl = make_plan(p);
     SFAST_REQUIRE(pl.nblk <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
     BlockAttnArgs a{};
-    a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.lse = lse;
+    a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.out_rest = out_rest, a.lse = lse;
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
     a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
     for (int i = 0; i < 3; ++i) a.qs[i] = p->qs[i], a.ks[i] = p->ks[i], a.vs[i] = p->vs[i], a.os[i] = p->os[i];

@@ -37,6 +37,11 @@ template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_ke
         unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.o + b * a.os[0] + s * a.os[1] + h * a.os[2] + d), y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
+        if (a.o_rest) {  // out to 16 more bits: in a row that attends to few keys dP - delta cancels
+            unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.o_rest + b * a.os[0] + s * a.os[1] + h * a.os[2] + d), y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
+        }
     }
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
@@ -389,13 +394,13 @@ extern "C" size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast
 }
 
 extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
-                                                  const int32_t *query_lengths, const void *out, const float *lse, const void *dout, const float *dlse,
-                                                  void *dq, void *dk, void *dv, const sfast_block_attn_params *p, void *workspace,
-                                                  size_t workspace_bytes, sfast_stream_t stream) {
+                                                  const int32_t *query_lengths, const void *out, const void *out_rest, const float *lse, const void *dout,
+                                                  const float *dlse, void *dq, void *dk, void *dv, const sfast_block_attn_params *p,
+                                                  void *workspace, size_t workspace_bytes, sfast_stream_t stream) {
     SFAST_REQUIRE(q && k && v && blocks && out && lse && dout && dq && dk && dv, SFAST_ERR_INVALID, "block_attention_backward: null argument");
     int rc = block_attn_check(p);
     if (rc != SFAST_OK) return rc;
-    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned8(dq) && aligned8(dk) && aligned8(dv),
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(dout) && aligned8(dq) && aligned8(dk) && aligned8(dv),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) {
         SFAST_REQUIRE(p->os[i] % 8 == 0 && p->dos[i] % 8 == 0 && p->os[i] >= 0 && p->dos[i] >= 0, SFAST_ERR_UNSUPPORTED,
@@ -410,7 +415,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_attention_backward: workspace too small");
     BlockAttnArgs a{};
-    a.q = q, a.k = k, a.v = v, a.o = out, a.dout = dout, a.lse = const_cast<float *>(lse), a.dlse = dlse, a.dq = dq, a.dk = dk, a.dv = dv;
+    a.q = q, a.k = k, a.v = v, a.o = out, a.o_rest = out_rest, a.dout = dout, a.lse = const_cast<float *>(lse), a.dlse = dlse, a.dq = dq, a.dk = dk, a.dv = dv;
     a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths;
     a.delta = (float *)workspace;
     a.cnt = (int32_t *)(a.delta + delta_floats(p));

@@ -10,4 +10,6 @@ __version__ = "0.1.0+mi355x"
 from . import torch_ops  # noqa: F401,E402  (torch.ops.sfast.*)
 from .triton import torch_ops as _triton_ops  # noqa: F401,E402  (torch.ops.sfast_triton.*)
 from .libs.xformers import xformers_attention as _xf_ops  # noqa: F401,E402  (torch.ops.sfast_xformers.*)
-from .libs.xformers import sparse_attention as _sparse_ops  # noqa: F401,E402  (block means / choice / attention)
+from .hip.lib import load_torch_ops as _load_torch_ops  # noqa: E402
+
+_load_torch_ops(required=False)  # native operators (positions, attention over chosen blocks); before the first build there are none

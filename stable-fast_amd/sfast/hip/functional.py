@@ -749,233 +749,51 @@ def qlinear_w8(x, w_int8, scale, bias=None, act=None):
     return out.reshape(*lead, N)
 
 
-# ---- video attention: positions over several axes, attention over chosen key blocks ------------------------------------------------
-_POS = {torch.int32: L.POS_I32, torch.int64: L.POS_I64, torch.float32: L.POS_F32, torch.float64: L.POS_F64}
-
-
-def _same_device(who, first, *rest):
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise L.SfastHipError(f"{who}: tensors on {first.device} and {t.device}")
-
-
-def _lengths(who, name, lengths, B, S, like):
-    """[B] sequence lengths as contiguous int32 (None: every sequence is full). Their values stay on the device; the kernels clip them."""
-    if lengths is None:
-        return None
-    if lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (B,):
-        raise L.SfastHipError(f"{who}: {name} must be {B} int32 or int64 values, got {lengths.dtype} {tuple(lengths.shape)}")
-    if lengths.dtype == torch.int64:
-        lengths = lengths.clamp(0, S).to(torch.int32)
-    return lengths.contiguous()
-
-
-def _i32(who, *sizes):
-    for n in sizes:
-        if n >= 1 << 31:
-            raise L.SfastHipError(f"{who}: a dimension of {n} is too long")
-
-
-@_on_device
+# ---- video attention: positions over several axes, attention over chosen key blocks. Native operators (csrc/torch/video_attention.cpp) -------
 def rotary_nd(q, k, positions, sections: Sequence[int], theta=10000.0, interleaved=True, inverse=False):
     """Rotary positions with several axes: axis a (time, height, width, ...) owns sections[a] consecutive elements of every head, pair i of it
     turns by positions[..., a] * theta ** (-2 i / sections[a]); elements behind the last section are copied.
 
-    q: [B, S, H, D], k: [B, S, Hk, D] or None (any strides; f16 / bf16 / f32); positions: [S, A] or [B, S, A] int32 / int64 / float32 /
-    float64. interleaved: pairs are neighbours, else the two halves of their section. inverse turns back, which is also the gradient.
-    Returns new tensors (q, k)."""
-    who = "rotary_nd"
-    _require_cuda(q, k, positions)
-    lib = L.init_device()
-    _same_device(who, q, k, positions)
-    if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
-        raise L.SfastHipError(f"{who}: expected q [B, S, H, D] and k [B, S, Hk, D] of one type")
-    B, S, H, D = q.shape
-    Hk = 0 if k is None else k.shape[2]
-    sections = [int(n) for n in sections]
-    if not 1 <= len(sections) <= L.ROPE_MAX_AXES:
-        raise L.SfastHipError(f"{who}: 1 to {L.ROPE_MAX_AXES} axes, got {len(sections)}")
-    if positions.dtype not in _POS:
-        raise L.SfastHipError(f"{who}: positions must be int32, int64, float32 or float64, got {positions.dtype}")
-    if positions.ndim == 2:
-        positions = positions.unsqueeze(0)
-    if positions.ndim != 3 or positions.shape[0] not in (1, B) or positions.shape[1] != S or positions.shape[2] != len(sections):
-        raise L.SfastHipError(f"{who}: positions must be [S, {len(sections)}] or [B, S, {len(sections)}], got {tuple(positions.shape)}")
-    if any(n <= 0 or n % 2 for n in sections) or sum(sections) > D:
-        raise L.SfastHipError(f"{who}: sections {sections} must be even, positive and fit the head dim {D}")
-    _i32(who, B, S, H, Hk, D)
-    dt = _dtype(q)
-
-    def fit(t):
-        # neighbouring pairs are read whole: rows start at even elements and pair-aligned addresses
-        if t is None or (t.stride(3) == 1 and not (interleaved and (any(st % 2 for st in t.stride()[:3]) or t.data_ptr() % (2 * t.element_size())))):
-            return t
-        return t.contiguous() if t.stride(3) != 1 or not t.is_contiguous() else t.clone()
-    q, k = fit(q), fit(k)
-    if positions.stride(2) != 1:
-        positions = positions.contiguous()
-    qo = torch.empty((B, S, H, D), dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty((B, S, Hk, D), dtype=q.dtype, device=q.device)
-    if qo.numel() == 0:
-        if ko is None or ko.numel() == 0:
-            return qo, ko
-        return qo, rotary_nd(k, None, positions, sections, theta, interleaved, inverse)[0]
-    zero = (0, 0, 0)
-    p = L.RopeParams(dt, B, S, H, Hk, D, len(sections), (C.c_int32 * L.ROPE_MAX_AXES)(*sections), int(bool(interleaved)), int(bool(inverse)),
-                     _POS[positions.dtype], float(theta), _i64x3(q.stride()[:3]), _i64x3(zero if k is None else k.stride()[:3]),
-                     _i64x3(qo.stride()[:3]), _i64x3(zero if ko is None else ko.stride()[:3]),
-                     (C.c_int64 * 2)(0 if positions.shape[0] == 1 else positions.stride(0), positions.stride(1)))
-    L.check(lib.sfast_hip_rope_nd(_ptr(q), _ptr(k), _ptr(positions), _ptr(qo), _ptr(ko), C.byref(p), _stream(q)), "sfast_hip_rope_nd")
-    return qo, ko
+    q: [B, S, H, D], k: [B, S, Hk, D] or None (any strides; f16 / bf16 / f32; D even, up to 256); positions: [S, A] or [B, S, A] int32 / int64 /
+    float32 / float64, 1 to 4 axes. interleaved: pairs are neighbours, else the two halves of their section. inverse turns back, which is also
+    the gradient. Returns new tensors (q, k). Differentiable in q and k."""
+    L.load_torch_ops()
+    return torch.ops.sfast.rotary_embedding_nd(q, k, positions, sections, theta, interleaved, inverse)
 
 
-@_on_device
 def block_means(x, block, lengths=None):
     """Means over blocks of `block` rows (1 to 1024): [B, S, H, D] (any strides; f16 / bf16 / f32) -> fp32 [B, ceil(S / block), H, D]. Rows from
-    lengths[b] on do not count; a block without rows gives zeros. Sums run in 64 bits."""
-    who = "block_means"
-    _require_cuda(x, lengths)
-    lib = L.init_device()
-    _same_device(who, x, lengths)
-    if x.ndim != 4:
-        raise L.SfastHipError(f"{who}: expected [B, S, H, D]")
-    if not 1 <= int(block) <= 1024:
-        raise L.SfastHipError(f"{who}: blocks of {block} rows (1 to 1024)")
-    B, S, H, D = x.shape
-    _i32(who, B, S, H * D)
-    lengths = _lengths(who, "lengths", lengths, B, S, x)
-    dt = _dtype(x)
-    if x.stride(3) != 1:
-        x = x.contiguous()
-    out = torch.empty((B, -(-S // int(block)), H, D), dtype=torch.float32, device=x.device)
-    if out.numel() == 0:
-        return out
-    p = L.BlockMeansParams(dt, B, S, H, D, int(block), _i64x3(x.stride()[:3]))
-    L.check(lib.sfast_hip_block_means(_ptr(x), _ptr(lengths), _ptr(out), C.byref(p), _stream(x)), "sfast_hip_block_means")
-    return out
+    lengths[b] on do not count; a block without rows gives zeros. Sums run in 64 bits. Takes no gradient."""
+    L.load_torch_ops()
+    return torch.ops.sfast_xformers.block_means(x, block, lengths)
 
 
-@_on_device
 def block_topk(query_means, key_means, topk, block_k=64, key_lengths=None):
     """The `topk` key blocks of every query block whose means agree best: fp32 [B, nQ, H, D] and [B, nK, Hk, D] -> int32 [B, Hk, nQ, topk].
     The score of a block is the sum of the products over the heads of a group, in 64 bits (the group shares its choice); blocks that begin
     at or behind key_lengths[b] (block_k keys each) do not take part. Ascending, -1 behind the last one; ties take the lowest block, a NaN
-    score ranks above all. nK <= 32768."""
-    who = "block_topk"
-    _require_cuda(query_means, key_means, key_lengths)
-    lib = L.init_device()
-    _same_device(who, query_means, key_means, key_lengths)
-    qm, km = query_means, key_means
-    if qm.ndim != 4 or km.ndim != 4 or qm.dtype != torch.float32 or km.dtype != torch.float32:
-        raise L.SfastHipError(f"{who}: expected fp32 means [B, nQ, H, D] and [B, nK, Hk, D]")
-    B, nQ, H, D = qm.shape
-    nK, Hk = km.shape[1], km.shape[2]
-    topk, block_k = int(topk), int(block_k)
-    if km.shape != (B, nK, Hk, D) or Hk == 0 or H % Hk:
-        raise L.SfastHipError(f"{who}: means {tuple(qm.shape)} and {tuple(km.shape)} do not fit")
-    if topk < 1 or block_k < 1:
-        raise L.SfastHipError(f"{who}: topk {topk} and block_k {block_k} must be positive")
-    _i32(who, topk, block_k)
-    key_lengths = _lengths(who, "key_lengths", key_lengths, B, min(nK * block_k, (1 << 31) - 1), qm)
-    out = torch.empty((B, Hk, nQ, topk), dtype=torch.int32, device=qm.device)
-    if out.numel() == 0:
-        return out
-    if nK == 0:
-        return out.fill_(-1)
-    qm, km = [t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (qm, km)]
-    p = L.BlockTopkParams(B, nQ, nK, H, Hk, D, topk, block_k)
-    ws, nb = _ws(lib.sfast_hip_block_topk_workspace_bytes(C.byref(p)), qm)
-    L.check(lib.sfast_hip_block_topk(_ptr(qm), _ptr(km), _ptr(key_lengths), _ptr(out), C.byref(p), _ptr(ws), nb, _stream(qm)), "sfast_hip_block_topk")
-    return out
+    score ranks above all. nK <= 32768, D % 4 == 0."""
+    L.load_torch_ops()
+    return torch.ops.sfast_xformers.block_topk(query_means, key_means, topk, block_k, key_lengths)
 
 
-def _rows16(t):
-    """The kernels read 16-byte runs of a row: head-dim stride 1, other strides multiples of 8, an aligned address, rows less than 2^23
-    elements apart. Anything else is copied."""
-    st = t.stride()
-    if st[3] == 1 and st[0] % 8 == 0 and st[1] % 8 == 0 and st[2] % 8 == 0 and t.data_ptr() % 16 == 0 and st[1] < 1 << 23:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _block_attention_params(who, q, k, v, blocks, block_q, block_k, key_lengths, query_lengths, scale):
-    _require_cuda(q, k, v, blocks, key_lengths, query_lengths)
-    _same_device(who, q, k, v, blocks, key_lengths, query_lengths)
-    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
-        raise L.SfastHipError(f"{who}: expected [B, S, H, D] tensors")
-    B, Sq, H, D = q.shape
-    Sk, Hk = k.shape[1], k.shape[2]
-    if k.shape != (B, Sk, Hk, D) or v.shape != k.shape or Hk == 0 or H % Hk or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise L.SfastHipError(f"{who}: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype} do not fit")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise L.SfastHipError(f"{who}: f16 / bf16 only, got {q.dtype}")
-    if D % 8 or not 8 <= D <= 128:
-        raise L.SfastHipError(f"{who}: head dim {D} (a multiple of 8 up to 128)")
-    if block_q not in (64, 128) or block_k not in (64, 128):
-        raise L.SfastHipError(f"{who}: blocks of 64 or 128 rows, got {block_q} and {block_k}")
-    nQ = -(-Sq // block_q)
-    if blocks.dtype != torch.int32 or blocks.ndim != 4 or tuple(blocks.shape[:3]) != (B, Hk, nQ):
-        raise L.SfastHipError(f"{who}: blocks must be int32 [{B}, {Hk}, {nQ}, topk], got {blocks.dtype} {tuple(blocks.shape)}")
-    scale = float(D) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise L.SfastHipError(f"{who}: the scale must be positive and finite, got {scale}")
-    _i32(who, B, Sq, Sk, H, blocks.shape[3])
-    p = L.BlockAttnParams()
-    p.dtype, p.B, p.H, p.Hk, p.Sq, p.Sk, p.D = _dtype(q), B, H, Hk, Sq, Sk, D
-    p.block_q, p.block_k, p.topk, p.scale = block_q, block_k, blocks.shape[3], scale
-    return p, blocks.contiguous(), _lengths(who, "key_lengths", key_lengths, B, Sk, q), _lengths(who, "query_lengths", query_lengths, B, Sq, q)
-
-
-@_on_device
 def block_sparse_attention(q, k, v, blocks, block_q=128, block_k=64, key_lengths=None, query_lengths=None, scale: Optional[float] = None):
     """softmax(scale q k^T) v over chosen key blocks: rows [i * block_q, ...) of q attend to the keys of blocks[b, hk, i, :] (block_k keys each).
 
-    q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] f16 / bf16, any strides; head h reads key head h // (H // Hk). blocks: int32 [B, Hk, nQ, topk], as
-    block_topk returns it: entries outside the sequence (-1) name nothing, an entry named twice counts twice. block_q, block_k: 64 or 128.
-    Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key, give zeros and lse = -inf.
-    scale: positive, default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq])."""
-    lib = L.init_device()
-    p, blocks, key_lengths, query_lengths = _block_attention_params("block_sparse_attention", q, k, v, blocks, int(block_q), int(block_k), key_lengths,
-                                                                    query_lengths, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((p.B, p.H, p.Sq), dtype=torch.float32, device=q.device)
-    if out.numel() == 0:
-        return out, lse
-    if p.Sk == 0 or p.topk == 0:
-        return out.zero_(), lse.fill_(float("-inf"))
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    p.qs, p.ks, p.vs, p.os = [_i64x3(t.stride()[:3]) for t in (q, k, v, out)]
-    ws, nb = _ws(lib.sfast_hip_block_attention_workspace_bytes(C.byref(p)), q)
-    rc = lib.sfast_hip_block_attention(_ptr(q), _ptr(k), _ptr(v), _ptr(blocks), _ptr(key_lengths), _ptr(query_lengths), _ptr(out), _ptr(lse),
-                                       C.byref(p), _ptr(ws), nb, _stream(q))
-    L.check(rc, "sfast_hip_block_attention")
-    return out, lse
+    q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] f16 / bf16, any strides, D % 8 == 0 up to 128; head h reads key head h // (H // Hk). blocks: int32
+    [B, Hk, ceil(Sq / block_q), topk], as block_topk returns it: entries outside the sequence (-1) name nothing, an entry named twice counts
+    twice. block_q, block_k: 64 or 128. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key, give
+    zeros and lse = -inf. scale: positive, default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq]). Differentiable once in q, k, v;
+    lse may carry a gradient too."""
+    L.load_torch_ops()
+    return torch.ops.sfast_xformers.block_sparse_attention(q, k, v, blocks, block_q, block_k, key_lengths, query_lengths, scale)
 
 
-@_on_device
 def block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q=128, block_k=64, key_lengths=None, query_lengths=None,
-                                    scale: Optional[float] = None):
-    """Gradients (dq, dk, dv) of block_sparse_attention from its results, the gradient of out and that of lse (or None). The same call gives the
+                                    scale: Optional[float] = None, out_rest=None):
+    """Gradients (dq, dk, dv) of block_sparse_attention from its results, the gradient of out and that of lse (or None). out_rest: what the
+    rounding of out left behind (autograd keeps it), without which rows that attend to few keys lose some accuracy. The same call gives the
     same bits."""
-    who = "block_sparse_attention_backward"
-    lib = L.init_device()
-    p, blocks, key_lengths, query_lengths = _block_attention_params(who, q, k, v, blocks, int(block_q), int(block_k), key_lengths, query_lengths, scale)
-    _require_cuda(grad_out, grad_lse, out, lse)
-    _same_device(who, q, grad_out, grad_lse, out, lse)
-    if grad_out.shape != q.shape or out.shape != q.shape or grad_out.dtype != q.dtype or out.dtype != q.dtype:
-        raise L.SfastHipError(f"{who}: out and its gradient must be like q")
-    stats = (p.B, p.H, p.Sq)
-    if tuple(lse.shape) != stats or lse.dtype != torch.float32 or (grad_lse is not None and (tuple(grad_lse.shape) != stats or grad_lse.dtype != torch.float32)):
-        raise L.SfastHipError(f"{who}: lse and its gradient must be fp32 {stats}")
-    dq, dk, dv = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-    if dq.numel() == 0 or dk.numel() == 0 or p.topk == 0:
-        return dq.zero_(), dk.zero_(), dv.zero_()
-    q, k, v, out, grad_out = [_rows16(t) for t in (q, k, v, out, grad_out)]
-    lse = lse.contiguous()
-    grad_lse = None if grad_lse is None else grad_lse.contiguous()
-    p.qs, p.ks, p.vs, p.os, p.dos, p.dqs, p.dks, p.dvs = [_i64x3(t.stride()[:3]) for t in (q, k, v, out, grad_out, dq, dk, dv)]
-    ws, nb = _ws(lib.sfast_hip_block_attention_backward_workspace_bytes(C.byref(p)), q)
-    rc = lib.sfast_hip_block_attention_backward(_ptr(q), _ptr(k), _ptr(v), _ptr(blocks), _ptr(key_lengths), _ptr(query_lengths), _ptr(out), _ptr(lse),
-                                                _ptr(grad_out), _ptr(grad_lse), _ptr(dq), _ptr(dk), _ptr(dv), C.byref(p), _ptr(ws), nb, _stream(q))
-    L.check(rc, "sfast_hip_block_attention_backward")
-    return dq, dk, dv
+    L.load_torch_ops()
+    return torch.ops.sfast_xformers.block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q, block_k, key_lengths,
+                                                                    query_lengths, scale, out_rest)

@@ -18,6 +18,9 @@ PROBES_LIB_PATH = os.path.join(os.path.dirname(_HERE), "_lib", "libsfast_hip_pro
 if os.environ.get("SFAST_HIP_PROBES", "0") == "1":
     LIB_PATH = PROBES_LIB_PATH
 
+# Native torch operators on the C ABI (csrc/torch/): registered by loading the file, which loads libsfast_hip.so beside it.
+TORCH_OPS_PATH = os.path.join(os.path.dirname(_HERE), "_lib", "libsfast_torch.so")
+
 ABI_VERSION = 10
 
 # enums (include/sfast_hip.h)
@@ -276,11 +279,11 @@ def _declare(lib):
     lib.sfast_hip_block_attention_workspace_bytes.restype = sz
     lib.sfast_hip_block_attention_workspace_bytes.argtypes = [C.POINTER(BlockAttnParams)]
     lib.sfast_hip_block_attention.restype = C.c_int
-    lib.sfast_hip_block_attention.argtypes = [vp] * 8 + [C.POINTER(BlockAttnParams), vp, sz, vp]
+    lib.sfast_hip_block_attention.argtypes = [vp] * 9 + [C.POINTER(BlockAttnParams), vp, sz, vp]
     lib.sfast_hip_block_attention_backward_workspace_bytes.restype = sz
     lib.sfast_hip_block_attention_backward_workspace_bytes.argtypes = [C.POINTER(BlockAttnParams)]
     lib.sfast_hip_block_attention_backward.restype = C.c_int
-    lib.sfast_hip_block_attention_backward.argtypes = [vp] * 13 + [C.POINTER(BlockAttnParams), vp, sz, vp]
+    lib.sfast_hip_block_attention_backward.argtypes = [vp] * 14 + [C.POINTER(BlockAttnParams), vp, sz, vp]
     lib.sfast_hip_cfg_ddim_step.restype = C.c_int
     lib.sfast_hip_cfg_ddim_step.argtypes = [vp, vp, vp, vp, vp, C.c_float, C.c_int64, C.c_int32, vp]
 
@@ -308,7 +311,28 @@ def load():
         if lib.sfast_hip_abi_version() != ABI_VERSION:
             raise SfastHipError("libsfast_hip.so ABI version mismatch; rebuild")
         _lib = lib
+    load_torch_ops()
     return _lib
+
+
+_torch_ops = False
+
+
+def load_torch_ops(required=True):
+    """Register the native operators (once). `required`: raise if they are not built, as load() does for the kernel library."""
+    global _torch_ops
+    if _torch_ops:
+        return True
+    with _lock:
+        if not _torch_ops:
+            if not os.path.exists(TORCH_OPS_PATH):
+                if required:
+                    raise SfastHipError(f"{TORCH_OPS_PATH} not found: build it with `python stable-fast_amd/build.py`. The native operators have no fallback.")
+                return False
+            import torch
+            torch.ops.load_library(TORCH_OPS_PATH)
+            _torch_ops = True
+    return True
 
 
 _probes_lib = None

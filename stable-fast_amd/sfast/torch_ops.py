@@ -285,37 +285,8 @@ _def("linear_relu(Tensor input, Tensor weight, Tensor? bias=None) -> Tensor", li
 _def("linear_gelu(Tensor input, Tensor weight, Tensor? bias=None) -> Tensor", linear_gelu)
 
 
-# ---- rotary positions with several axes (no counterpart in the reference) -------------------------------------------------------------
-def rotary_embedding_nd(query, key, positions, sections, theta=10000.0, interleaved=True, inverse=False):
-    """Turns the pairs of every head of query [B, S, H, D] and key [B, S, Hk, D] by their axis' position: what a transformer over images or
-    video does before attention (`sfast_xformers::memory_efficient_attention`, `::block_sparse_attention`). See hip.functional.rotary_nd."""
-    return F.rotary_nd(query, key, positions, sections, theta, interleaved, inverse)
-
-
-_def("rotary_embedding_nd(Tensor query, Tensor key, Tensor positions, int[] sections, float theta=10000.0, bool interleaved=True, "
-     "bool inverse=False) -> (Tensor, Tensor)", rotary_embedding_nd)
-
-
-def _rotary_setup(ctx, inputs, output):
-    _, _, positions, *ctx.rotary = inputs
-    ctx.save_for_backward(positions)
-    ctx.set_materialize_grads(False)
-
-
-def _rotary_backward(ctx, grad_query, grad_key):
-    """A turn is orthogonal: its gradient is the turn back (positions take no gradient)."""
-    positions, = ctx.saved_tensors
-    sections, theta, interleaved, inverse = ctx.rotary
-    if grad_query is not None and grad_key is not None:
-        grad_query, grad_key = torch.ops.sfast.rotary_embedding_nd(grad_query, grad_key, positions, sections, theta, interleaved, not inverse)
-    elif grad_query is not None:
-        grad_query = F.rotary_nd(grad_query, None, positions, sections, theta, interleaved, not inverse)[0]
-    elif grad_key is not None:
-        grad_key = F.rotary_nd(grad_key, None, positions, sections, theta, interleaved, not inverse)[0]
-    return grad_query, grad_key, None, None, None, None, None
-
-
-torch.library.register_autograd("sfast::rotary_embedding_nd", _rotary_backward, setup_context=_rotary_setup)
+# ---- rotary positions with several axes (no counterpart in the reference): `sfast::rotary_embedding_nd` is a native operator, registered by
+# csrc/torch/video_attention.cpp when the package is imported; hip.functional.rotary_nd says what it does -------------------------------------
 
 
 # ---- int8 dynamic linear (reference csrc/operators/cutlass/cutlass_qlinear.cc:10-89) ---------------------------------------------

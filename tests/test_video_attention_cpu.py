@@ -51,9 +51,9 @@ def test_block_attention_refuses_before_it_launches(built_lib, over, code):
     lib = L.load()
     p = attn_params(L, **over)
     ptr = 4096   # an aligned address that nothing reads
-    assert lib.sfast_hip_block_attention(ptr, ptr, ptr, ptr, None, None, ptr, ptr, C.byref(p), ptr, 1 << 40, None) == code
+    assert lib.sfast_hip_block_attention(ptr, ptr, ptr, ptr, None, None, ptr, ptr, None, C.byref(p), ptr, 1 << 40, None) == code
     assert b"block_attention" in lib.sfast_hip_last_error()
-    assert lib.sfast_hip_block_attention_backward(ptr, ptr, ptr, ptr, None, None, ptr, ptr, ptr, None, ptr, ptr, ptr, C.byref(p), ptr, 1 << 40, None) == code
+    assert lib.sfast_hip_block_attention_backward(ptr, ptr, ptr, ptr, None, None, ptr, None, ptr, ptr, None, ptr, ptr, ptr, C.byref(p), ptr, 1 << 40, None) == code
 
 
 def test_block_attention_refuses_addresses_and_workspaces(built_lib):
@@ -64,21 +64,21 @@ def test_block_attention_refuses_addresses_and_workspaces(built_lib):
     assert need > 0 and need % 4 == 0
     good = [4096] * 8
     for at in (0, 1, 2, 3, 6, 7):      # q, k, v, blocks, out, lse
-        args = [4096, 4096, 4096, 4096, None, None, 4096, 4096]
+        args = [4096, 4096, 4096, 4096, None, None, 4096, 4096, None]
         args[at] = None
         assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, need, None) == -2
     for at in (0, 1, 2):
-        args = [4096, 4096, 4096, 4096, None, None, 4096, 4096]
+        args = [4096, 4096, 4096, 4096, None, None, 4096, 4096, None]
         args[at] = 4098
         assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, need, None) == -1
-    args = good[:4] + [None, None, 4096, 4096]
+    args = good[:4] + [None, None, 4096, 4096, None]
     assert lib.sfast_hip_block_attention(*args, C.byref(p), None, 0, None) == -3
     assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, need - 1, None) == -3
     need = lib.sfast_hip_block_attention_backward_workspace_bytes(C.byref(p))
     assert need >= (2 * 4 * 1 + 2 * 2 * 1 * 8) * 4
-    back = [4096, 4096, 4096, 4096, None, None, 4096, 4096, 4096, None, 4096, 4096, 4096]
+    back = [4096, 4096, 4096, 4096, None, None, 4096, None, 4096, 4096, None, 4096, 4096, 4096]
     assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, need - 1, None) == -3
-    for at in (0, 3, 6, 7, 8, 10, 11, 12):
+    for at in (0, 3, 6, 8, 9, 11, 12, 13):
         args = list(back)
         args[at] = None
         assert lib.sfast_hip_block_attention_backward(*args, C.byref(p), 4096, need, None) == -2

@@ -274,21 +274,23 @@ def test_block_attention_odd_lists(case, grads):
 def test_block_attention_does_not_read_behind_the_sequences(case, grads):
     B, Sq, Sk, H, Hk, D, bq, bk, topk, kl, ql = case
     q, k, v, blocks = make(case, F16, 5)
-    want = attend(case, q, k, v, blocks, grads=grads)
+    attend(case, q, k, v, blocks, grads=grads)
     go = randn((B, Sq, H, D), F16, 77)
+
+    def results():
+        leaves = [t.detach().requires_grad_(grads) for t in (q, k, v)]
+        out, lse = ATT.block_sparse_attention(*leaves, blocks, bq, bk, lens(kl), lens(ql))
+        if not grads:
+            return out, lse
+        gl = torch.where(torch.isfinite(lse.detach()), randn((B, H, Sq), F32, 78), 0.0)
+        return torch.autograd.grad((out, torch.where(torch.isfinite(lse.detach()), lse, 0.0)), leaves, (go, gl))
+    want = results()
     for b in range(B):
         k[b, R.clip(kl, b, Sk):] = float("nan")
         v[b, R.clip(kl, b, Sk):] = float("inf")
         q[b, R.clip(ql, b, Sq):] = float("nan")
         go[b, R.clip(ql, b, Sq):] = float("nan")
-    if not grads:
-        got = ATT.block_sparse_attention(q, k, v, blocks, bq, bk, lens(kl), lens(ql))
-    else:
-        leaves = [t.requires_grad_() for t in (q, k, v)]
-        out, lse = ATT.block_sparse_attention(*leaves, blocks, bq, bk, lens(kl), lens(ql))
-        gl = torch.where(torch.isfinite(lse.detach()), randn((B, H, Sq), F32, 78), 0.0)
-        got = torch.ops.sfast_xformers.block_sparse_attention_backward(go, gl, q, k, v, blocks, out.detach(), lse.detach(), bq, bk, lens(kl), lens(ql))
-    for g, w in zip(got, want):
+    for g, w in zip(results(), want):
         assert torch.equal(g, w)
 
 
@@ -344,6 +346,42 @@ def test_block_attention_gradient_of_an_expanded_and_of_an_unused_result():
     want = R.attention(q.detach(), k.detach(), v.detach(), blocks, bq, bk, kl, ql, None, torch.zeros_like(out), gl)
     for name, g in zip(("dq", "dk", "dv"), got):
         R.check(name, g, *want[name])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_row_with_one_key_has_no_score_gradient(dtype):
+    """One key: P = 1 and dP = delta, so dq = dk = 0 but for what rowsum(dO O) is off: the step of out's rest (u^2) and the fp32 sums. A rounded
+    out alone would leave u."""
+    B, Sq, Sk, H, D = 2, 70, 129, 2, 64
+    q, k, v, go = [randn((B, n, H, D), dtype, i) for i, n in enumerate((Sq, Sk, Sk, Sq))]
+    blocks = torch.full((B, H, 1, 1), 2, dtype=torch.int32, device="cuda")   # the block that holds key 128 alone
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out, lse = ATT.block_sparse_attention(*leaves, blocks)
+    dq, dk, dv = torch.autograd.grad(out, leaves, go)
+    last_k, last_v = k.detach()[:, 128:].double(), v.detach()[:, 128:].double()
+    assert torch.equal(out.detach(), v.detach()[:, 128:].expand_as(out))
+    u = R.half_step(dtype)
+    off = (go.double().abs() * last_v.abs()).sum(-1, keepdim=True) * (u * u + (2 * D + 8) * R.U32) * (1 + u) * D ** -0.5
+    R.check("dq", dq, torch.zeros_like(dq, dtype=torch.float64), off * last_k.abs() + R.tiny(dtype))
+    assert (dk[:, :128] == 0).all() and (dv[:, :128] == 0).all()
+    R.check("dk", dk[:, 128:], torch.zeros_like(last_k), (off * q.detach().double().abs()).sum(1, keepdim=True) + R.tiny(dtype))
+    total = go.double().sum(1, keepdim=True)
+    R.check("dv", dv[:, 128:], total, u * total.abs() + Sq * R.U32 * 2 * go.double().abs().sum(1, keepdim=True))
+
+
+def test_there_is_no_second_derivative():
+    q, k, v, blocks = make(CASES[1], BF16)
+    q.requires_grad_()
+    out, _ = ATT.block_sparse_attention(q, k, v, blocks, 128, 64)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(out.sum(), q, create_graph=True)
+    x = randn((1, 6, 1, 8), F32, 1).requires_grad_()          # a turn has one: it is linear in what it turns
+    y, none = OPS.rotary_embedding_nd(x, None, grid(1, 2, 3, 1), [8])
+    assert none is None
+    g, = torch.autograd.grad((y ** 3).sum(), x, create_graph=True)
+    h, = torch.autograd.grad(g.sum(), x)
+    assert torch.isfinite(h).all() and (h != 0).any()
+    assert not ATT.block_means(x, 64).requires_grad
 
 
 def test_block_attention_gradients_against_differences():
@@ -435,7 +473,8 @@ def test_a_clip_through_positions_choice_and_attention(dtype):
     want = R.attention(qd, kd, v.detach(), blocks, 128, 64, kl, grad_out=go)
     R.check("dv", got[2], *want["dv"])
     # the turn back of the gradients that attention gave
-    d = torch.ops.sfast_xformers.block_sparse_attention_backward(go, None, qd, kd, v.detach(), blocks, out.detach(), lse.detach(), 128, 64, lens(kl))
+    alone = [a.detach().requires_grad_() for a in (qd, kd, v)]
+    d = torch.autograd.grad(ATT.block_sparse_attention(*alone, blocks, 128, 64, lens(kl))[0], alone, go)
     back = OPS.rotary_embedding_nd(d[0], d[1], pos, sections, 10000.0, True, True)
     assert torch.equal(got[0], back[0]) and torch.equal(got[1], back[1])
 
