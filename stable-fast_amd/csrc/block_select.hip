@@ -28,16 +28,16 @@ template <typename T, int V> __global__ void __launch_bounds__(256) block_means_
     __shared__ double part[8][32 * V];
     const int tid = threadIdx.x, col = tid & 31, grp = tid >> 5;
     const int cols = (a.runs + 31) / 32;
-    const int64_t unit = blockIdx.x / cols;
-    const int run = (int)(blockIdx.x - unit * cols) * 32 + col;
-    const int j = (int)(unit % a.n), b = (int)(unit / a.n);
+    const int unit = (int)(blockIdx.x / (uint32_t)cols);
+    const int run = (int)(blockIdx.x - (uint32_t)unit * cols) * 32 + col;
+    const int b = unit / a.n, j = unit - b * a.n;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
-    const int rows = min(max(len - j * a.block, 0), a.block);
+    const int rows = min(max(len - j * a.block, 0), a.block);  // (j * block <= S)
     double sum[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0;
-    const int64_t e = (int64_t)run * V;
-    const int h = (int)(e / a.D), d = (int)(e - (int64_t)h * a.D);
+    const int e = run * V;  // H * D has 31 bits
+    const int h = e / a.D, d = e - h * a.D;
     if (run < a.runs) {
         const T *x = (const T *)a.x + b * a.xs[0] + (int64_t)j * a.block * a.xs[1] + h * a.xs[2] + d;
         int r = grp;
@@ -60,14 +60,14 @@ template <typename T, int V> __global__ void __launch_bounds__(256) block_means_
     for (int i = 0; i < V; ++i) part[grp][i * 32 + col] = sum[i];
     __syncthreads();
     // output element i of run c: the workgroup's 32 * V elements are neighbours in memory
-    const int64_t first = (int64_t)(blockIdx.x - unit * cols) * 32 * V;
+    const int first = (int)(blockIdx.x - (uint32_t)unit * cols) * 32 * V;
     for (int i = tid; i < 32 * V; i += 256) {
         const int c = i / V, k = i - c * V;
-        if (first + i >= (int64_t)a.H * a.D) continue;
+        if (first + i >= a.H * a.D) continue;
         double s = 0.0;
 #pragma unroll
         for (int g = 0; g < 8; ++g) s += part[g][k * 32 + c];
-        a.out[unit * a.H * a.D + first + i] = rows > 0 ? (float)(s / rows) : 0.f;
+        a.out[(int64_t)unit * a.H * a.D + first + i] = rows > 0 ? (float)(s / rows) : 0.f;
     }
 }
 
@@ -87,11 +87,11 @@ struct TopkArgs {
 
 __device__ __forceinline__ int topk_count(const TopkArgs &a, int b) {
     if (!a.klen) return a.nK;
-    const int64_t n = ((int64_t)max(a.klen[b], 0) + a.bk - 1) / a.bk;
-    return (int)min(n, (int64_t)a.nK);
+    const uint32_t n = ((uint32_t)max(a.klen[b], 0) + (uint32_t)(a.bk - 1)) / (uint32_t)a.bk;
+    return (int)min(n, (uint32_t)a.nK);
 }
 
-template <int MI, int NJ> __global__ void __launch_bounds__(256) block_score_kernel(const TopkArgs a) {
+template <int MI, int NJ> __global__ void __launch_bounds__(256, 4) block_score_kernel(const TopkArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4;
     const int pair = blockIdx.z, hk = pair % a.Hk, b = pair / a.Hk;
     const int i0 = blockIdx.y * 16 * MI, j0 = (blockIdx.x * 4 + wave) * 16 * NJ;
@@ -102,37 +102,51 @@ template <int MI, int NJ> __global__ void __launch_bounds__(256) block_score_ker
     for (int x = 0; x < MI; ++x)
 #pragma unroll
         for (int y = 0; y < NJ; ++y) acc[x][y] = f64x4{0.0, 0.0, 0.0, 0.0};
+    // rows outside read row 0: their products land in results that nobody stores
+    const float *kp[NJ], *qp[MI];
+#pragma unroll
+    for (int y = 0; y < NJ; ++y) {
+        const int j = j0 + 16 * y + l15;
+        kp[y] = a.km + (((int64_t)b * a.nK + (j < count ? j : 0)) * a.Hk + hk) * a.D + 4 * l4;
+    }
+#pragma unroll
+    for (int x = 0; x < MI; ++x) {
+        const int i = i0 + 16 * x + l15;
+        qp[x] = a.qm + (((int64_t)b * a.nQ + (i < a.nQ ? i : 0)) * a.H + hk * a.G) * a.D + 4 * l4;
+    }
+    f32x4 k[NJ], q[MI];
+    const auto load = [&](int d0) __attribute__((always_inline)) {
+        const bool in = d0 + 4 * l4 < a.D;
+#pragma unroll
+        for (int y = 0; y < NJ; ++y) k[y] = in ? *reinterpret_cast<const f32x4 *>(kp[y] + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < MI; ++x) q[x] = in ? *reinterpret_cast<const f32x4 *>(qp[x] + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    load(0);
     for (int d0 = 0; d0 < a.D; d0 += 16) {
-        const int d = d0 + 4 * l4;
-        double q[MI][4], k[NJ][4];
+        double kd[NJ][4], qd[MI][4];
 #pragma unroll
-        for (int y = 0; y < NJ; ++y) {
-            const int j = j0 + 16 * y + l15;
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            if (d < a.D && j < count) v = *reinterpret_cast<const f32x4 *>(a.km + (((int64_t)b * a.nK + j) * a.Hk + hk) * a.D + d);
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) k[y][t] = (double)v[t];
+            for (int y = 0; y < NJ; ++y) kd[y][t] = (double)k[y][t];
+#pragma unroll
+            for (int x = 0; x < MI; ++x) qd[x][t] = (double)q[x][t];
         }
+        const bool in = d0 + 4 * l4 < a.D;
+        for (int g = 1; g < a.G; ++g)
 #pragma unroll
-        for (int x = 0; x < MI; ++x) {
-            const int i = i0 + 16 * x + l15;
+            for (int x = 0; x < MI; ++x) {
+                const f32x4 v = in ? *reinterpret_cast<const f32x4 *>(qp[x] + (int64_t)g * a.D + d0) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 4; ++t) q[x][t] = 0.0;
-            if (d < a.D && i < a.nQ) {
-                const float *row = a.qm + (((int64_t)b * a.nQ + i) * a.H + hk * a.G) * a.D + d;
-                for (int g = 0; g < a.G; ++g) {
-                    const f32x4 v = *reinterpret_cast<const f32x4 *>(row + g * a.D);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) q[x][t] += (double)v[t];
-                }
+                for (int t = 0; t < 4; ++t) qd[x][t] += (double)v[t];
             }
-        }
+        if (d0 + 16 < a.D) load(d0 + 16);  // under the products of this group
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int x = 0; x < MI; ++x)
 #pragma unroll
-                for (int y = 0; y < NJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f64_16x16x4f64(q[x][t], k[y][t], acc[x][y], 0, 0, 0);
+                for (int y = 0; y < NJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f64_16x16x4f64(qd[x][t], kd[y][t], acc[x][y], 0, 0, 0);
     }
     // result register r of a lane: query block 4 r + lane / 16, key block lane % 16
 #pragma unroll
@@ -150,10 +164,65 @@ template <int MI, int NJ> __global__ void __launch_bounds__(256) block_score_ker
         }
 }
 
+// One or a few query blocks (a token): bound by reading the key means, not worth a matrix tile. Eight lanes share a key block (128 bytes of its
+// row at a time), a wave holds 32 key blocks in registers, and the query sums wait in LDS as 64-bit numbers.
+constexpr int SCORE_FEW = 4, SCORE_FEW_D = 128;
+__global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) {
+    __shared__ __attribute__((aligned(16))) double qs[SCORE_FEW][SCORE_FEW_D];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l7 = lane & 7, l8 = lane >> 3;
+    const int pair = blockIdx.z, hk = pair % a.Hk, b = pair / a.Hk;
+    const int count = topk_count(a, b);
+    const int j0 = (blockIdx.x * 4 + wave) * 32;
+    if ((int)blockIdx.x * 128 >= count) return;
+    f32x4 k[4][4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+        const int j = j0 + 8 * y + l8;
+        const float *row = a.km + (((int64_t)b * a.nK + (j < count ? j : 0)) * a.Hk + hk) * a.D;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = 32 * c + 4 * l7;
+            k[y][c] = d < a.D ? *reinterpret_cast<const f32x4 *>(row + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    for (int e = tid; e < a.nQ * a.D; e += 256) {
+        const int i = e / a.D, d = e - i * a.D;
+        const float *q = a.qm + (((int64_t)b * a.nQ + i) * a.H + hk * a.G) * a.D + d;
+        double s = 0.0;
+        for (int g = 0; g < a.G; ++g) s += (double)q[(int64_t)g * a.D];
+        qs[i][d] = s;
+    }
+    __syncthreads();
+    for (int i = 0; i < a.nQ; ++i) {
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int d = 32 * c + 4 * l7;
+            if (d < a.D) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const double q = qs[i][d + t];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) s[y] = fma(q, (double)k[y][c][t], s[y]);
+                }
+            }
+        }
+        double *row = a.score + ((int64_t)pair * a.nQ + i) * a.nK;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+#pragma unroll
+            for (int off = 4; off >= 1; off >>= 1) s[y] += __shfl_xor(s[y], off, 64);
+            const int j = j0 + 8 * y + l8;
+            if (l7 == 0 && j < count) row[j] = s[y];
+        }
+    }
+}
+
 // ---- the topk best of a row ---------------------------------------------------------------------------------------------------------------
 // WAVES waves hold a row's scores in registers as order-preserving 64-bit keys (0 = not there) and find the topk-th largest bit by bit from
-// the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. Keys equal to the
-// threshold are taken in the order of their index.
+// the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. It starts below the
+// bits that all keys share and looks at the upper 32 bits first: those settle all but near-ties, for two instructions a key and bit. Keys
+// equal to the threshold are taken in the order of their index.
 __device__ __forceinline__ uint64_t topk_key(double s) {
     s += 0.0;  // -0 and 0 are one score
     const uint64_t u = __builtin_bit_cast(uint64_t, s);
@@ -161,52 +230,107 @@ __device__ __forceinline__ uint64_t topk_key(double s) {
     return (u >> 63) ? ~u : (u | (1ull << 63));
 }
 
-template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) block_topk_kernel(const TopkArgs a, int64_t n_rows) {
-    __shared__ int sums[2][WAVES], above_s[WAVES], equal_s[WAVES];
+// sum / maximum over a wave, the same in every lane (row shifts by 1, 2, 4, 8, then across the rows of 16: lane 63 holds the result)
+template <int CTRL> __device__ __forceinline__ uint32_t topk_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ uint32_t topk_wave_sum(uint32_t v) {
+    v += topk_dpp<0x111>(v), v += topk_dpp<0x112>(v), v += topk_dpp<0x114>(v), v += topk_dpp<0x118>(v);
+    v += topk_dpp<0x142>(v), v += topk_dpp<0x143>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t topk_wave_max(uint32_t v) {
+    v = max(v, topk_dpp<0x111>(v)), v = max(v, topk_dpp<0x112>(v)), v = max(v, topk_dpp<0x114>(v)), v = max(v, topk_dpp<0x118>(v));
+    v = max(v, topk_dpp<0x142>(v)), v = max(v, topk_dpp<0x143>(v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) block_topk_kernel(const TopkArgs a, int n_rows) {
+    __shared__ uint32_t sums[2][WAVES];
+    __shared__ int above_s[WAVES], equal_s[WAVES];
     const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
-    const int64_t row = WAVES == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-    if (row >= n_rows) return;
-    const int64_t pair = row / a.nQ;
-    const int count = topk_count(a, (int)(pair / a.Hk));
+    const int row_id = (int)(WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);  // up to 2^30 rows
+    if (row_id >= n_rows) return;
+    const int64_t row = row_id;
+    const int count = topk_count(a, row_id / a.nQ / a.Hk);
     const int j0 = wave * 64 * NPL + lane;
-    uint64_t key[NPL];
+    uint32_t hi[NPL], lo[NPL];
+    double score[NPL];
 #pragma unroll
-    for (int n = 0; n < NPL; ++n) key[n] = j0 + 64 * n < count ? topk_key(a.score[row * a.nK + j0 + 64 * n]) : 0ull;
+    for (int n = 0; n < NPL; ++n) score[n] = a.score[row * a.nK + min(j0 + 64 * n, a.nK - 1)];  // all in flight, whether they count or not
+#pragma unroll
+    for (int n = 0; n < NPL; ++n) {
+        const uint64_t k = j0 + 64 * n < count ? topk_key(score[n]) : 0ull;
+        hi[n] = (uint32_t)(k >> 32), lo[n] = (uint32_t)k;
+    }
     int turn = 0;
-    const auto total = [&](int mine) -> int {
+    const auto over_waves = [&](uint32_t mine, bool most) __attribute__((always_inline)) -> uint32_t {
         if (WAVES == 1) return mine;
         turn ^= 1;
         if (lane == 0) sums[turn][wave] = mine;
         __syncthreads();
-        int s = 0;
+        uint32_t s = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) s += sums[turn][w];
+        for (int w = 0; w < WAVES; ++w) s = most ? max(s, sums[turn][w]) : s + sums[turn][w];
         return s;
     };
-    uint64_t edge = 1;     // keys above it (or at it, in order) are chosen
-    int at_edge = 0;       // how many of those at it; 0: all
+    uint32_t edge_hi = 0, edge_lo = 1;  // keys above it (or at it, in order) are chosen
+    int at_edge = 0;                    // how many of those at it; 0: all
     if (count > a.topk) {
-        edge = 0;
-        bool exact = false;
-        for (int bit = 63; bit >= 0; --bit) {
-            const uint64_t cand = edge | (1ull << bit);
-            int mine = 0;
+        const uint32_t want = (uint32_t)a.topk;
+        uint32_t big = 0, small = 0;    // largest upper half, largest complement of one (of a key that is there)
 #pragma unroll
-            for (int n = 0; n < NPL; ++n) mine += __popcll(__ballot(key[n] >= cand));
-            const int have = total(mine);
-            if (have >= a.topk) edge = cand;
-            if (have == a.topk) {
+        for (int n = 0; n < NPL; ++n) {
+            big = max(big, hi[n]);
+            small = max(small, j0 + 64 * n < count ? ~hi[n] : 0u);
+        }
+        big = over_waves(topk_wave_max(big), true);
+        small = ~over_waves(topk_wave_max(small), true);
+        const uint32_t differ = big ^ small;
+        bool exact = false;
+        edge_lo = 0;
+        const int top = differ ? 31 - __builtin_clz(differ) : -1;
+        edge_hi = top == 31 ? 0u : top < 0 ? big : big & ~((2u << top) - 1u);
+        for (int bit = top; bit >= 0; --bit) {
+            const uint32_t cand = edge_hi | (1u << bit);
+            uint32_t mine = 0;
+#pragma unroll
+            for (int n = 0; n < NPL; ++n) mine += hi[n] >= cand ? 1u : 0u;
+            const uint32_t have = over_waves(topk_wave_sum(mine), false);
+            if (have >= want) edge_hi = cand;
+            if (have == want) {
                 exact = true;
                 break;
             }
         }
         if (!exact) {
-            int mine = 0;
+            // the topk-th key has this upper half; how many lie above it, then the lower half among its equals
+            uint32_t mine = 0;
 #pragma unroll
-            for (int n = 0; n < NPL; ++n) mine += __popcll(__ballot(key[n] > edge));
-            at_edge = a.topk - total(mine);
+            for (int n = 0; n < NPL; ++n) mine += hi[n] > edge_hi ? 1u : 0u;
+            const uint32_t above = over_waves(topk_wave_sum(mine), false);
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t cand = edge_lo | (1u << bit);
+                mine = 0;
+#pragma unroll
+                for (int n = 0; n < NPL; ++n) mine += hi[n] == edge_hi && lo[n] >= cand ? 1u : 0u;
+                const uint32_t have = above + over_waves(topk_wave_sum(mine), false);
+                if (have >= want) edge_lo = cand;
+                if (have == want) {
+                    exact = true;
+                    break;
+                }
+            }
+            if (!exact) {
+                mine = 0;
+#pragma unroll
+                for (int n = 0; n < NPL; ++n) mine += hi[n] == edge_hi && lo[n] > edge_lo ? 1u : 0u;
+                at_edge = (int)(want - above - over_waves(topk_wave_sum(mine), false));
+            }
         }
     }
+    const uint64_t edge = ((uint64_t)edge_hi << 32) | edge_lo;
+    const auto key = [&](int n) __attribute__((always_inline)) { return ((uint64_t)hi[n] << 32) | lo[n]; };
     // positions: chosen keys of earlier waves, earlier registers, lower lanes
     const uint64_t below = (1ull << lane) - 1;
     int above0 = 0, equal0 = 0;
@@ -214,8 +338,8 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
         int ab = 0, eq = 0;
 #pragma unroll
         for (int n = 0; n < NPL; ++n) {
-            ab += __popcll(__ballot(key[n] > edge));
-            eq += __popcll(__ballot(key[n] == edge));
+            ab += __popcll(__ballot(key(n) > edge));
+            eq += __popcll(__ballot(key(n) == edge));
         }
         if (lane == 0) above_s[wave] = ab, equal_s[wave] = eq;
         __syncthreads();
@@ -225,9 +349,9 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
     int32_t *out = a.out + row * a.topk;
 #pragma unroll
     for (int n = 0; n < NPL; ++n) {
-        const uint64_t ab = __ballot(key[n] > edge), eq = __ballot(key[n] == edge);
+        const uint64_t ab = __ballot(key(n) > edge), eq = __ballot(key(n) == edge);
         const int rank = equal0 + __popcll(eq & below);
-        const bool take = key[n] > edge || (key[n] == edge && rank < limit);
+        const bool take = key(n) > edge || (key(n) == edge && rank < limit);
         if (take) out[above0 + __popcll(ab & below) + min(rank, limit)] = j0 + 64 * n;
         above0 += __popcll(ab);
         equal0 += __popcll(eq);
@@ -238,7 +362,7 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
 template <int WAVES, int NPL> int launch_topk(const TopkArgs &a, hipStream_t st) {
     const int64_t rows = (int64_t)a.B * a.Hk * a.nQ;
     const dim3 grid((unsigned)(WAVES == 1 ? ceil_div64(rows, 4) : rows));
-    hipLaunchKernelGGL((block_topk_kernel<WAVES, NPL>), grid, dim3(WAVES == 1 ? 256 : WAVES * 64), 0, st, a, rows);
+    hipLaunchKernelGGL((block_topk_kernel<WAVES, NPL>), grid, dim3(WAVES == 1 ? 256 : WAVES * 64), 0, st, a, (int)rows);
     return check_launch("block_topk");
 }
 
@@ -258,7 +382,7 @@ static int check_topk(const sfast_block_topk_params *p) {
 template <typename T> static int means_launch(MeansArgs &a, int run, hipStream_t st) {
     a.runs = a.H * (a.D / run);
     const int64_t blocks = (int64_t)a.B * a.n * ceil_div(a.runs, 32);
-    SFAST_REQUIRE(blocks <= (1ll << 31) - 1, SFAST_ERR_UNSUPPORTED, "block_means: too many blocks");
+    SFAST_REQUIRE(blocks <= (1ll << 31) - 1 && (int64_t)a.H * a.D <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_means: too many blocks");
     const dim3 grid((unsigned)blocks);
     set_kernel_name("block_means[V=%d]", run);
     constexpr int MOST = 16 / sizeof(T);
@@ -314,8 +438,11 @@ extern "C" int sfast_hip_block_topk(const float *qm, const float *km, const int3
     a.B = p->B, a.nQ = p->nQ, a.nK = p->nK, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.D = p->D, a.topk = p->topk, a.bk = p->block_k;
     hipStream_t st = (hipStream_t)stream;
     const unsigned pairs = (unsigned)(p->B * p->Hk);
-    // up to 16 query blocks (a token has one): one row tile, the four waves side by side along the key blocks
-    if (p->nQ <= 16)
+    // a few query blocks (a token has one): the key means are read once, no matrix tile; up to 16: one row tile, the four waves side by side
+    // along the key blocks
+    if (p->nQ <= SCORE_FEW && p->D <= SCORE_FEW_D)
+        hipLaunchKernelGGL(block_score_few_kernel, dim3((unsigned)ceil_div(p->nK, 128), 1, pairs), dim3(256), 0, st, a);
+    else if (p->nQ <= 16)
         hipLaunchKernelGGL((block_score_kernel<1, 1>), dim3((unsigned)ceil_div(p->nK, 64), 1, pairs), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((block_score_kernel<2, 2>), dim3((unsigned)ceil_div(p->nK, 128), (unsigned)ceil_div(p->nQ, 32), pairs), dim3(256), 0, st, a);

@@ -152,12 +152,13 @@ extern "C" int sfast_hip_rope_nd(const void *q, const void *k, const void *posit
     int run = 16 / es;  // elements of one access
     const auto fits = [&](int64_t v) { while (run > 1 && v % run) run >>= 1; };
     int at = 0;
+    const double octaves = log2(p->theta);
     for (int x = 0; x < p->n_axes; ++x) {
         const int d = p->sections[x];
         SFAST_REQUIRE(d > 0 && d % 2 == 0 && d <= p->D - at, SFAST_ERR_INVALID, "rope_nd: section %d has %d of %d elements left (even, positive)", x, d,
                       p->D - at);
         a.half0[x] = at / 2;
-        for (int i = 0; i < d / 2; ++i) a.turn[at / 2 + i] = pow(p->theta, -2.0 * i / d) / (2.0 * M_PI);
+        for (int i = 0; i < d / 2; ++i) a.turn[at / 2 + i] = exp2(-2.0 * i / d * octaves) * (0.5 / M_PI);
         if (!p->interleaved) fits(d / 2);
         at += d;
     }
