@@ -96,14 +96,30 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
             kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, Kn, wave);
             vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, Kn + TILE, wave);
         }
+        // scores: all K fragments are requested before the first product (the two key halves alternate: independent accumulators)
+        vec8 kf[2][KD];
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) kf[kb][kd] = ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi);
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 sc[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
 #pragma unroll
-            for (int kd = 0; kd < KD; ++kd) sc[kb] = ba_mfma(ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi), qf[kd], sc[kb]);
-        }
+        for (int kd = 0; kd < KD; ++kd)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) sc[kb] = ba_mfma(kf[kb][kd], qf[kd], sc[kb]);
+        __builtin_amdgcn_sched_barrier(0);
+        // V^T fragments of the first half of the keys arrive under the softmax
+        vec8 vf[4][DB];
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, g * 16);
+        __builtin_amdgcn_sched_barrier(0);
         const int left = klen - cur * 64;
         if (left < 64) {
 #pragma unroll
@@ -140,10 +156,15 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
                 l += e;
                 p[kb * 2 + (i >> 3)][i & 7] = Elem<T>::from_f32(e);
             }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int g = 2; g < 4; ++g)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) o[db] = ba_mfma(ba_col_frag<T, DP>(Vs, lane, db, g * 16), p[g], o[db]);
+            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, g * 16);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] = ba_mfma(vf[g][db], p[g], o[db]);
     }
     l = ba_xor32_sum(l);
     if (!inside) return;
