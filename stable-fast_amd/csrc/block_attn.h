@@ -123,8 +123,9 @@ __device__ __forceinline__ float ba_xor32_sum(float v) {
 
 // Every wave's LDS-DMA requests have landed and every wave is done reading what the next requests overwrite. (The compiler's barrier waits
 // for LDS operations, not for LDS-DMA: that wait is spelled out.)
-__device__ __forceinline__ void ba_sync() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+// LEFT: requests of this wave that may still be on their way (they return in order).
+template <int LEFT = 0> __device__ __forceinline__ void ba_sync() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT > 63 ? 63 : LEFT) : "memory");
     __syncthreads();
 }
 
@@ -133,6 +134,7 @@ __device__ __forceinline__ void ba_sync() {
 __device__ __forceinline__ int ba_tiles(const int32_t *list, int e0, int e1, int bk, int klen, int lane, int *tiles) {
     int n = 0;
     const int sub = bk >> 6;
+#pragma unroll 1
     for (int e = e0; e < e1; e += 64) {
         const int j = e + lane < e1 ? list[e + lane] : -1;
         const int64_t first = (int64_t)j * bk;

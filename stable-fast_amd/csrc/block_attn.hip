@@ -9,6 +9,7 @@
 //   * few query rows (a token against a long cache): the rows of all heads of a group share a wave (the group shares its list, K and V are
 //     read once), and a list is split over workgroups whose partial results a second launch joins.
 #include "block_attn.h"
+#include <type_traits>
 
 namespace sfast {
 
@@ -16,15 +17,16 @@ namespace {
 
 constexpr int BA_MAX_LIST = 1024;  // entries of one workgroup's (part of a) list: 2048 tiles
 
-template <int DP> constexpr int ba_fwd_lds() { return 4 * BaTile<DP>::BYTES + BA_MAX_LIST * 2 * 4 + 16; }
+template <int DP, int NS> constexpr int ba_fwd_lds() { return NS * 2 * BaTile<DP>::BYTES + BA_MAX_LIST * 2 * 4 + 16; }
 
+// NS: LDS stages, NS - 1 tiles are on their way while one is used.
 // PACK: rows are (query, head of the group) pairs, row = s * G + g, one unit per key head; else one unit per query head.
-template <typename T, int DP, int NW, bool PACK>
+template <typename T, int DP, int NW, int NS, bool PACK>
 __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int *tiles = reinterpret_cast<int *>(smem + 4 * TILE);
+    int *tiles = reinterpret_cast<int *>(smem + NS * 2 * TILE);
     int *ntiles_p = tiles + 2 * BA_MAX_LIST;
 
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
@@ -81,21 +83,24 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
 
     __syncthreads();
     const int n = __builtin_amdgcn_readfirstlane(*ntiles_p);
-    int next = n > 0 ? __builtin_amdgcn_readfirstlane(tiles[0]) : 0;
-    if (n > 0) {
-        kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, smem, wave);
-        vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, smem + TILE, wave);
-    }
+    const auto request = [&](int t) __attribute__((always_inline)) {
+        const int tile = __builtin_amdgcn_readfirstlane(tiles[t]);
+        char *st = smem + (t % NS) * (2 * TILE);
+        kl.load(Kp, a.ks[1], a.D, tile * 64, klen - tile * 64, st, wave);
+        vl.load(Vp, a.vs[1], a.D, tile * 64, klen - tile * 64, st + TILE, wave);
+    };
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < n) request(t);
     for (int t = 0; t < n; ++t) {
-        const int cur = next;
-        char *Ks = smem + (t & 1) * (2 * TILE), *Vs = Ks + TILE;
-        if (t + 1 < n) next = __builtin_amdgcn_readfirstlane(tiles[t + 1]);
-        ba_sync();  // tile t has landed, every wave is done with the other stage
-        if (t + 1 < n) {
-            char *Kn = smem + ((t + 1) & 1) * (2 * TILE);
-            kl.load(Kp, a.ks[1], a.D, next * 64, klen - next * 64, Kn, wave);
-            vl.load(Vp, a.vs[1], a.D, next * 64, klen - next * 64, Kn + TILE, wave);
-        }
+        const int cur = __builtin_amdgcn_readfirstlane(tiles[t]);
+        char *Ks = smem + (t % NS) * (2 * TILE), *Vs = Ks + TILE;
+        // tile t has landed (NS - 2 later ones may be on their way), every wave is done with the stage that is requested next
+        if (NS > 2 && t + NS - 2 < n)
+            ba_sync<(NS - 2) * 2 * BaLoader<DP, NW>::N>();
+        else
+            ba_sync();
+        if (t + NS - 1 < n) request(t + NS - 1);
         // scores: all K fragments are requested before the first product (the two key halves alternate: independent accumulators)
         vec8 kf[2][KD];
 #pragma unroll
@@ -215,49 +220,60 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
     }
 }
 
-// joins the parts of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. One wave a row.
-template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_attn_join_kernel(const BlockAttnArgs a, int rows) {
+// joins the parts of a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. One wave a row: lane p has part p's weight (64 parts at a time),
+// every lane two columns, eight parts in flight.
+template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_attn_join_kernel(const BlockAttnArgs a, int rows, int n_rows) {
     const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);   // (b, hk, qb, g, row of the block) | (b, hk, row)
+    const int id = blockIdx.x * 4 + (threadIdx.x >> 6);   // (b, hk, qb, g, row of the block) | (b, hk, row)
+    if (id >= n_rows) return;
     const int per = PACK ? a.Sq * a.G : a.bq;
-    const int64_t unit = id / per;
-    const int r = (int)(id - unit * per);
-    int64_t x = unit;
-    const int g = PACK ? 0 : (int)(x % a.G);
-    if (!PACK) x /= a.G;
-    const int qb = PACK ? 0 : (int)(x % a.nQ);
-    if (!PACK) x /= a.nQ;
-    const int hk = (int)(x % a.Hk), b = (int)(x / a.Hk);
-    if (b >= a.B) return;
+    const int unit = id / per, r = id - unit * per;
+    int x = unit, g = 0, qb = 0;
+    if (!PACK) g = x % a.G, x /= a.G, qb = x % a.nQ, x /= a.nQ;
+    const int b = x / a.Hk, hk = x - b * a.Hk;
     const int s = PACK ? r / a.G : qb * a.bq + r;
     const int h = hk * a.G + (PACK ? r - s * a.G : g);
     if (s >= a.Sq) return;
-    const float *ml = a.part_ml + (unit * a.nsplit * rows + r) * 2;
-    const int64_t step = (int64_t)rows;
-    float M = -INFINITY, L = 0.f;
-    for (int p = lane; p < a.nsplit; p += 64) M = fmaxf(M, ml[p * step * 2]);
-    M = wave_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int p = lane; p < a.nsplit; p += 64) L += __builtin_amdgcn_exp2f(ml[p * step * 2] - ref) * ml[p * step * 2 + 1];
-    L = wave_sum(L);
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    const float *po = a.part_o + (unit * a.nsplit * rows + r) * a.D;
-    const int64_t at = (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
-    T *Op = (T *)a.out + at;
-    for (int d = lane * 2; d < a.D; d += 128) {
-        float x0 = 0.f, x1 = 0.f;
-        for (int p = 0; p < a.nsplit; ++p) {
-            const float w = __builtin_amdgcn_exp2f(ml[p * step * 2] - ref);
-            const float2 v = *reinterpret_cast<const float2 *>(po + p * step * a.D + d);
-            x0 = fmaf(w, v.x, x0);
-            x1 = fmaf(w, v.y, x1);
+    const int64_t first = (int64_t)unit * a.nsplit * rows + r;
+    const float *ml = a.part_ml + first * 2;
+    const float *po = a.part_o + first * a.D;
+    const int64_t ml_step = (int64_t)rows * 2, po_step = (int64_t)rows * a.D;
+    const int d = lane * 2 < a.D ? lane * 2 : 0;
+    float M = -INFINITY, L = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int p0 = 0; p0 < a.nsplit; p0 += 64) {
+        const int n = min(64, a.nsplit - p0);
+        float2 mine = make_float2(-INFINITY, 0.f);
+        if (lane < n) mine = *reinterpret_cast<const float2 *>(ml + (p0 + lane) * ml_step);
+        const float top = fmaxf(M, wave_max(mine.x));
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float old = __builtin_amdgcn_exp2f(M - ref);  // (-inf: nothing was summed yet)
+        const float w = __builtin_amdgcn_exp2f(mine.x - ref);
+        M = top;
+        L = L * old + wave_sum(w * mine.y);
+        x0 *= old, x1 *= old;
+#pragma unroll 1
+        for (int p = 0; p < n; p += 8) {
+            float2 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const float2 *>(po + (int64_t)(p0 + min(p + i, n - 1)) * po_step + d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float wi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), min(p + i, 63)));
+                if (p + i >= n) wi = 0.f, v[i] = make_float2(0.f, 0.f);
+                x0 = fmaf(wi, v[i].x, x0);
+                x1 = fmaf(wi, v[i].y, x1);
+            }
         }
+    }
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const int64_t at = (int64_t)b * a.os[0] + (int64_t)s * a.os[1] + (int64_t)h * a.os[2];
+    if (lane * 2 < a.D) {
         const T y0 = Elem<T>::from_f32(x0 * inv), y1 = Elem<T>::from_f32(x1 * inv);
-        Op[d] = y0;
-        Op[d + 1] = y1;
+        const typename Elem<T>::vec2 y = {y0, y1};
+        *reinterpret_cast<typename Elem<T>::vec2 *>((T *)a.out + at + d) = y;
         if (a.out_rest) {
-            ((T *)a.out_rest)[at + d] = Elem<T>::from_f32(x0 * inv - (float)y0);
-            ((T *)a.out_rest)[at + d + 1] = Elem<T>::from_f32(x1 * inv - (float)y1);
+            const typename Elem<T>::vec2 z = {Elem<T>::from_f32(x0 * inv - (float)y0), Elem<T>::from_f32(x1 * inv - (float)y1)};
+            *reinterpret_cast<typename Elem<T>::vec2 *>((T *)a.out_rest + at + d) = z;
         }
     }
     if (lane == 0) {
@@ -267,9 +283,9 @@ template <typename T, bool PACK> __global__ void __launch_bounds__(256) block_at
     }
 }
 
-template <typename T, int DP, int NW, bool PACK> int set_attr() {
-    auto kern = block_attn_fwd_kernel<T, DP, NW, PACK>;
-    const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, ba_fwd_lds<DP>());
+template <typename T, int DP, int NW, int NS, bool PACK> int set_attr() {
+    auto kern = block_attn_fwd_kernel<T, DP, NW, NS, PACK>;
+    const hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, ba_fwd_lds<DP, NS>());
     if (e != hipSuccess) {
         set_error("hipFuncSetAttribute(block_attn_fwd): %s", hipGetErrorString(e));
         return SFAST_ERR_LAUNCH;
@@ -278,13 +294,16 @@ template <typename T, int DP, int NW, bool PACK> int set_attr() {
 }
 
 struct Plan {
-    bool pack;
+    bool pack, deep;
     int nw, nsplit;
     int64_t units, nblk;
 };
 
-// How a call is cut into workgroups. Packed rows: all query rows of a group fit 64 rows of one or two waves. A list is split when the
-// query blocks alone would leave compute units empty: 512 workgroups are two on each, and a part keeps at least two tiles.
+// How a call is cut into workgroups.
+//  * Packed rows: all query rows of a group fit 64 rows of one or two waves.
+//  * A list is split over workgroups where that is shorter. Measured: a workgroup takes 1.1 us a tile while compute units are free (512
+//    workgroups are two on each); a split adds 4 us for the second launch and the partial results' way through memory at 0.8 bytes / ps.
+//  * deep: four LDS stages instead of two, for grids that leave one workgroup to a compute unit anyway.
 static Plan make_plan(const sfast_block_attn_params *p) {
     Plan pl{};
     const int G = p->H / p->Hk;
@@ -293,39 +312,53 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     pl.nw = pl.pack ? (p->Sq * G <= 32 ? 1 : 2) : p->block_q / 32;
     pl.units = (int64_t)p->B * p->Hk * nQ * (pl.pack ? 1 : G);
     const int64_t tiles = (int64_t)p->topk * (p->block_k / 64);
-    int64_t ns = 1;
-    if (pl.units < 256) ns = ceil_div64(512, pl.units);
-    if (ns > tiles / 2) ns = tiles / 2;
-    if (ns > p->topk) ns = p->topk;
-    if (ns < 1) ns = 1;
     const int64_t least = ceil_div64(p->topk, BA_MAX_LIST - 1);  // a part holds at most BA_MAX_LIST entries
-    if (ns < least) ns = least;
+    int64_t ns = least;
+    if (pl.units < 256) {
+        const double rows = pl.pack ? (double)p->Sq * G : pl.nw * 32;
+        const double part = 2.0 * pl.units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
+        double best = 1.1 * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
+        for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * pl.units <= 1024; ++x) {
+            const double rounds = (double)ceil_div64(x * pl.units, 512);
+            const double t = 1.1 * (double)ceil_div64(tiles, x) * rounds + 4.0 + part * (double)x;
+            if (t < best) best = t, ns = x;
+        }
+    }
     pl.nsplit = (int)ns;
     pl.nblk = pl.units * ns;
+    pl.deep = pl.nblk <= 256;
     return pl;
 }
 
 template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl, hipStream_t st) {
     const dim3 grid((unsigned)(8 * a.chunk));
-    const size_t lds = ba_fwd_lds<DP>();
-    if (pl.pack) {
-        if (pl.nw == 1)
-            hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 1, true>), grid, dim3(64), lds, st, a);
+    const auto go = [&](auto NW, auto NS, auto PACK) {
+        constexpr int nw = decltype(NW)::value, ns = decltype(NS)::value;
+        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * 64), (ba_fwd_lds<DP, ns>()), st, a);
+    };
+    const auto with = [&](auto NW, auto PACK) {
+        if (pl.deep)
+            go(NW, std::integral_constant<int, 4>{}, PACK);
         else
-            hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 2, true>), grid, dim3(128), lds, st, a);
-    } else if (pl.nw == 2) {
-        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 2, false>), grid, dim3(128), lds, st, a);
-    } else {
-        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, 4, false>), grid, dim3(256), lds, st, a);
-    }
+            go(NW, std::integral_constant<int, 2>{}, PACK);
+    };
+    if (pl.pack && pl.nw == 1)
+        with(std::integral_constant<int, 1>{}, std::true_type{});
+    else if (pl.pack)
+        with(std::integral_constant<int, 2>{}, std::true_type{});
+    else if (pl.nw == 2)
+        with(std::integral_constant<int, 2>{}, std::false_type{});
+    else
+        with(std::integral_constant<int, 4>{}, std::false_type{});
     int rc = check_launch("block_attention");
     if (rc || pl.nsplit == 1) return rc;
     const int per = pl.pack ? a.Sq * a.G : a.bq;
-    const dim3 jgrid((unsigned)ceil_div64(pl.units * per, 4));
+    const int rows = (int)(pl.units * per);  // (a split call has few units)
+    const dim3 jgrid((unsigned)ceil_div(rows, 4));
     if (pl.pack)
-        hipLaunchKernelGGL((block_attn_join_kernel<T, true>), jgrid, dim3(256), 0, st, a, pl.nw * 32);
+        hipLaunchKernelGGL((block_attn_join_kernel<T, true>), jgrid, dim3(256), 0, st, a, pl.nw * 32, rows);
     else
-        hipLaunchKernelGGL((block_attn_join_kernel<T, false>), jgrid, dim3(256), 0, st, a, pl.nw * 32);
+        hipLaunchKernelGGL((block_attn_join_kernel<T, false>), jgrid, dim3(256), 0, st, a, pl.nw * 32, rows);
     return check_launch("block_attention join");
 }
 
@@ -351,11 +384,15 @@ int block_attn_check(const sfast_block_attn_params *p) {
 
 int block_attn_init() {
     int rc = 0;
-#define SFAST_BA_ATTR(T, DP)                         \
-    if (!rc) rc = set_attr<T, DP, 1, true>();        \
-    if (!rc) rc = set_attr<T, DP, 2, true>();        \
-    if (!rc) rc = set_attr<T, DP, 2, false>();       \
-    if (!rc) rc = set_attr<T, DP, 4, false>();
+#define SFAST_BA_ATTR(T, DP)                                                         \
+    if (!rc) rc = set_attr<T, DP, 1, 2, true>();                                     \
+    if (!rc) rc = set_attr<T, DP, 2, 2, true>();                                     \
+    if (!rc) rc = set_attr<T, DP, 2, 2, false>();                                    \
+    if (!rc) rc = set_attr<T, DP, 4, 2, false>();                                    \
+    if (!rc) rc = set_attr<T, DP, 1, 4, true>();                                     \
+    if (!rc) rc = set_attr<T, DP, 2, 4, true>();                                     \
+    if (!rc) rc = set_attr<T, DP, 2, 4, false>();                                    \
+    if (!rc) rc = set_attr<T, DP, 4, 4, false>();
     SFAST_BA_ATTR(f16, 64)
     SFAST_BA_ATTR(f16, 128)
     SFAST_BA_ATTR(bf16, 64)
@@ -384,7 +421,7 @@ extern "C" int sfast_hip_block_attention(const void *q, const void *k, const voi
     SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out) && aligned8(out_rest), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) SFAST_REQUIRE(p->os[i] % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_attention: output strides must be multiples of 4 elements");
     const Plan pl = make_plan(p);
-    SFAST_REQUIRE(pl.nblk <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
+    SFAST_REQUIRE(pl.nblk <= (1ll << 30) && pl.nblk * (pl.nsplit > 1 ? 128 : 1) <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
     BlockAttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.out_rest = out_rest, a.lse = lse;
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
@@ -402,7 +439,8 @@ extern "C" int sfast_hip_block_attention(const void *q, const void *k, const voi
         a.part_ml = a.part_o + (size_t)pl.nblk * (pl.nw * 32) * p->D;
     }
     hipStream_t st = (hipStream_t)stream;
-    set_kernel_name("block_attn_fwd[DP=%d,rows=%d,split=%d%s]", p->D <= 64 ? 64 : 128, pl.nw * 32, pl.nsplit, pl.pack ? ",packed" : "");
+    set_kernel_name("block_attn_fwd[DP=%d,rows=%d,stages=%d,split=%d%s]", p->D <= 64 ? 64 : 128, pl.nw * 32, pl.deep ? 4 : 2, pl.nsplit,
+                    pl.pack ? ",packed" : "");
     if (p->dtype == SFAST_F16) return p->D <= 64 ? launch<f16, 64>(a, pl, st) : launch<f16, 128>(a, pl, st);
     return p->D <= 64 ? launch<bf16, 64>(a, pl, st) : launch<bf16, 128>(a, pl, st);
 }
