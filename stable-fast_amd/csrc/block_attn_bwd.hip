@@ -146,13 +146,28 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
             const int left = klen - cur * 64;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                // all fragments of a product are requested ahead of it, K^T's under the exponentials
+                vec8 kf[KD], vf[KD], kt[2][DB];
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) {
+                    kf[kd] = ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi);
+                    vf[kd] = ba_row_frag<T, DP>(Vs, kb * 32 + l31, kd, hi);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 f32x16 sc, dp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) sc = ba_mfma(ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi), qf[kd], sc);
+                for (int kd = 0; kd < KD; ++kd) {
+                    sc = ba_mfma(kf[kd], qf[kd], sc);
+                    dp = ba_mfma(vf[kd], gf[kd], dp);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) dp = ba_mfma(ba_row_frag<T, DP>(Vs, kb * 32 + l31, kd, hi), gf[kd], dp);
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) kt[g][db] = ba_col_frag<T, DP>(Ks, lane, db, kb * 32 + g * 16);
+                __builtin_amdgcn_sched_barrier(0);
                 if (left < 64) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -165,9 +180,9 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                     ds[i >> 3][i & 7] = Elem<T>::from_f32(p * (dp[i] - delta));
                 }
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
+                for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) dq[db] = ba_mfma(ba_col_frag<T, DP>(Ks, lane, db, kb * 32 + g * 16), ds[g], dq[db]);
+                    for (int db = 0; db < DB; ++db) dq[db] = ba_mfma(kt[g][db], ds[g], dq[db]);
             }
         }
     }
@@ -275,13 +290,30 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
             if (x + 1 < steps) request(x + 1, (x + 1) & 1);
 #pragma unroll
             for (int rb = 0; rb < 2; ++rb) {
+                vec8 qf[KD], gf[KD], qt[2][DB], gt[2][DB];
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) {
+                    qf[kd] = ba_row_frag<T, DP>(Qs, rb * 32 + l31, kd, hi);
+                    gf[kd] = ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 f32x16 sc, dp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) sc = ba_mfma(ba_row_frag<T, DP>(Qs, rb * 32 + l31, kd, hi), kf[kd], sc);
+                for (int kd = 0; kd < KD; ++kd) {
+                    sc = ba_mfma(qf[kd], kf[kd], sc);
+                    dp = ba_mfma(gf[kd], vf[kd], dp);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) dp = ba_mfma(ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi), vf[kd], dp);
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        gt[g][db] = ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16);
+                        qt[g][db] = ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
                 vec8 p8[2], ds[2];
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) {
@@ -296,11 +328,11 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                     }
                 }
 #pragma unroll
-                for (int db = 0; db < DB; ++db)
+                for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        dv[db] = ba_mfma(ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16), p8[g], dv[db]);
-                        dk[db] = ba_mfma(ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16), ds[g], dk[db]);
+                    for (int db = 0; db < DB; ++db) {
+                        dv[db] = ba_mfma(gt[g][db], p8[g], dv[db]);
+                        dk[db] = ba_mfma(qt[g][db], ds[g], dk[db]);
                     }
             }
         }
