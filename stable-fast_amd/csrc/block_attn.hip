@@ -311,15 +311,17 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     pl.pack = nQ == 1 && (int64_t)p->Sq * G <= 64;
     pl.nw = pl.pack ? (p->Sq * G <= 32 ? 1 : 2) : p->block_q / 32;
     pl.units = (int64_t)p->B * p->Hk * nQ * (pl.pack ? 1 : G);
+    // (SFAST_BATCH_INVARIANT: a sample's parts are those of the reference batch, common.h)
+    const int64_t units = g_batch_ref > 0 ? pl.units / p->B * g_batch_ref : pl.units;
     const int64_t tiles = (int64_t)p->topk * (p->block_k / 64);
     const int64_t least = ceil_div64(p->topk, BA_MAX_LIST - 1);  // a part holds at most BA_MAX_LIST entries
     int64_t ns = least;
-    if (pl.units < 256) {
+    if (units < 256) {
         const double rows = pl.pack ? (double)p->Sq * G : pl.nw * 32;
-        const double part = 2.0 * pl.units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
+        const double part = 2.0 * units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
         double best = 1.1 * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
-        for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * pl.units <= 1024; ++x) {
-            const double rounds = (double)ceil_div64(x * pl.units, 512);
+        for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * units <= 1024; ++x) {
+            const double rounds = (double)ceil_div64(x * units, 512);
             const double t = 1.1 * (double)ceil_div64(tiles, x) * rounds + 4.0 + part * (double)x;
             if (t < best) best = t, ns = x;
         }

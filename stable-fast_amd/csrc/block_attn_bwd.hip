@@ -15,11 +15,11 @@ namespace sfast {
 
 namespace {
 
-constexpr int BB_LIST = 1024;  // list entries held in LDS at a time
+constexpr int BB_LIST = 1024, BB_NAMES = 256;  // list entries, query blocks held in LDS at a time (four dkv workgroups of D <= 64 fit a compute unit)
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 16; }
-template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 2 * 2 * 64 * 4 + 16; }
+template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + BB_NAMES * 2 * 4 + 2 * 2 * 64 * 4 + 16; }
 
 // delta of a row: 16 lanes, 8 elements each
 template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a) {
@@ -206,7 +206,7 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, NT = NW * 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int *names = reinterpret_cast<int *>(smem + 4 * TILE);       // query block, count of it
-    float *stat = reinterpret_cast<float *>(names + 2 * BB_LIST);  // two stages of 64 (lse in log2 units - log2 count), 64 delta
+    float *stat = reinterpret_cast<float *>(names + 2 * BB_NAMES);  // two stages of 64 (lse in log2 units - log2 count), 64 delta
     int *n_p = reinterpret_cast<int *>(stat + 2 * 2 * 64);
 
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
@@ -267,12 +267,12 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
     };
 
     const int i_all = (int64_t)j * a.bk < klen ? (qlen + a.bq - 1) / a.bq : 0;
-    for (int i0 = 0; i0 < i_all; i0 += BB_LIST) {
+    for (int i0 = 0; i0 < i_all; i0 += BB_NAMES) {
         __syncthreads();
         if (wave == 0) {
             int n = 0;
-            for (int i = i0; i < min(i0 + BB_LIST, i_all); i += 64) {
-                const int m = i + lane < min(i0 + BB_LIST, i_all) ? cnt[i + lane] : 0;
+            for (int i = i0; i < min(i0 + BB_NAMES, i_all); i += 64) {
+                const int m = i + lane < min(i0 + BB_NAMES, i_all) ? cnt[i + lane] : 0;
                 const uint64_t some = __ballot(m > 0);
                 const int at = n + __popcll(some & ((1ull << lane) - 1));
                 if (m > 0) names[2 * at] = i + lane, names[2 * at + 1] = m;

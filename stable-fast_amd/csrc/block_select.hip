@@ -221,8 +221,8 @@ __global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) 
 // ---- the topk best of a row ---------------------------------------------------------------------------------------------------------------
 // WAVES waves hold a row's scores in registers as order-preserving 64-bit keys (0 = not there) and find the topk-th largest bit by bit from
 // the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. It starts below the
-// bits that all keys share and looks at the upper 32 bits first: those settle all but near-ties, for two instructions a key and bit. Keys
-// equal to the threshold are taken in the order of their index.
+// bits that all keys share and looks at the upper 31 bits first: those settle all but near-ties, for two instructions a key and bit (a
+// comparison's mask would cost wait states on top). Keys equal to the threshold are taken in the order of their index.
 __device__ __forceinline__ uint64_t topk_key(double s) {
     s += 0.0;  // -0 and 0 are one score
     const uint64_t u = __builtin_bit_cast(uint64_t, s);
@@ -254,14 +254,15 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
     const int64_t row = row_id;
     const int count = topk_count(a, row_id / a.nQ / a.Hk);
     const int j0 = wave * 64 * NPL + lane;
-    uint32_t hi[NPL], lo[NPL];
+    uint64_t key[NPL];
+    uint32_t up[NPL];  // the upper 31 bits
     double score[NPL];
 #pragma unroll
     for (int n = 0; n < NPL; ++n) score[n] = a.score[row * a.nK + min(j0 + 64 * n, a.nK - 1)];  // all in flight, whether they count or not
 #pragma unroll
     for (int n = 0; n < NPL; ++n) {
-        const uint64_t k = j0 + 64 * n < count ? topk_key(score[n]) : 0ull;
-        hi[n] = (uint32_t)(k >> 32), lo[n] = (uint32_t)k;
+        key[n] = j0 + 64 * n < count ? topk_key(score[n]) : 0ull;
+        up[n] = (uint32_t)(key[n] >> 33);
     }
     int turn = 0;
     const auto over_waves = [&](uint32_t mine, bool most) __attribute__((always_inline)) -> uint32_t {
@@ -274,89 +275,98 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
         for (int w = 0; w < WAVES; ++w) s = most ? max(s, sums[turn][w]) : s + sums[turn][w];
         return s;
     };
-    uint32_t edge_hi = 0, edge_lo = 1;  // keys above it (or at it, in order) are chosen
-    int at_edge = 0;                    // how many of those at it; 0: all
-    if (count > a.topk) {
+    int32_t *out = a.out + row * a.topk;
+    for (int i = count + (WAVES == 1 ? lane : (int)threadIdx.x); i < a.topk; i += WAVES == 1 ? 64 : WAVES * 64) out[i] = -1;
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t edge_up = 0;
+    bool exact = count <= a.topk;  // everything that is there is chosen (and is not 0 in its upper bits: only keys that are not there are)
+    if (!exact) {
         const uint32_t want = (uint32_t)a.topk;
-        uint32_t big = 0, small = 0;    // largest upper half, largest complement of one (of a key that is there)
+        uint32_t big = 0, small = 0;  // largest upper part, largest complement of one (of a key that is there)
 #pragma unroll
         for (int n = 0; n < NPL; ++n) {
-            big = max(big, hi[n]);
-            small = max(small, j0 + 64 * n < count ? ~hi[n] : 0u);
+            big = max(big, up[n]);
+            small = max(small, j0 + 64 * n < count ? ~up[n] : 0u);
         }
         big = over_waves(topk_wave_max(big), true);
         small = ~over_waves(topk_wave_max(small), true);
         const uint32_t differ = big ^ small;
-        bool exact = false;
-        edge_lo = 0;
         const int top = differ ? 31 - __builtin_clz(differ) : -1;
-        edge_hi = top == 31 ? 0u : top < 0 ? big : big & ~((2u << top) - 1u);
+        edge_up = big & ~((2u << top) - 1u);
+        if (top < 0) edge_up = big;
         for (int bit = top; bit >= 0; --bit) {
-            const uint32_t cand = edge_hi | (1u << bit);
-            uint32_t mine = 0;
+            const uint32_t cand = edge_up | (1u << bit);
+            // 31-bit numbers: the sign of the difference tells which is less; the signs are collected and counted at the end
+            uint32_t less = 0;
 #pragma unroll
-            for (int n = 0; n < NPL; ++n) mine += hi[n] >= cand ? 1u : 0u;
-            const uint32_t have = over_waves(topk_wave_sum(mine), false);
-            if (have >= want) edge_hi = cand;
+            for (int n = 0; n < NPL; ++n) less = __builtin_amdgcn_alignbit(less, up[n] - cand, 31);
+            const uint32_t have = (uint32_t)(64 * NPL * WAVES) - over_waves(topk_wave_sum(__builtin_popcount(less)), false);
+            if (have >= want) edge_up = cand;
             if (have == want) {
                 exact = true;
                 break;
             }
         }
-        if (!exact) {
-            // the topk-th key has this upper half; how many lie above it, then the lower half among its equals
-            uint32_t mine = 0;
-#pragma unroll
-            for (int n = 0; n < NPL; ++n) mine += hi[n] > edge_hi ? 1u : 0u;
-            const uint32_t above = over_waves(topk_wave_sum(mine), false);
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t cand = edge_lo | (1u << bit);
-                mine = 0;
-#pragma unroll
-                for (int n = 0; n < NPL; ++n) mine += hi[n] == edge_hi && lo[n] >= cand ? 1u : 0u;
-                const uint32_t have = above + over_waves(topk_wave_sum(mine), false);
-                if (have >= want) edge_lo = cand;
-                if (have == want) {
-                    exact = true;
-                    break;
-                }
-            }
-            if (!exact) {
-                mine = 0;
-#pragma unroll
-                for (int n = 0; n < NPL; ++n) mine += hi[n] == edge_hi && lo[n] > edge_lo ? 1u : 0u;
-                at_edge = (int)(want - above - over_waves(topk_wave_sum(mine), false));
-            }
-        }
     }
-    const uint64_t edge = ((uint64_t)edge_hi << 32) | edge_lo;
-    const auto key = [&](int n) __attribute__((always_inline)) { return ((uint64_t)hi[n] << 32) | lo[n]; };
-    // positions: chosen keys of earlier waves, earlier registers, lower lanes
-    const uint64_t below = (1ull << lane) - 1;
+    if (exact) {
+        // positions: chosen keys of earlier waves, earlier registers, lower lanes
+        const uint32_t from = max(edge_up, 1u);
+        int at = 0;
+        if (WAVES > 1) {
+            int mine = 0;
+#pragma unroll
+            for (int n = 0; n < NPL; ++n) mine += __popcll(__ballot(up[n] >= from));
+            if (lane == 0) above_s[wave] = mine;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) at += above_s[w];
+        }
+#pragma unroll
+        for (int n = 0; n < NPL; ++n) {
+            const bool take = up[n] >= from;
+            const uint64_t some = __ballot(take);
+            if (take) out[at + __popcll(some & below)] = j0 + 64 * n;
+            at += __popcll(some);
+        }
+        return;
+    }
+    // Scores that agree in their upper 31 bits stand at the border: the topk-th key has the upper bits edge_up; the other 33 decide, then the index.
+    const uint32_t want = (uint32_t)a.topk;
+    uint64_t edge = (uint64_t)edge_up << 33;
+    const auto reach = [&](uint64_t from) __attribute__((always_inline)) -> uint32_t {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int n = 0; n < NPL; ++n) mine += key[n] >= from ? 1u : 0u;
+        return over_waves(topk_wave_sum(mine), false);
+    };
+    bool all = false;  // exactly topk keys reach the edge
+    for (int bit = 32; bit >= 0 && !all; --bit) {
+        const uint64_t cand = edge | (1ull << bit);
+        const uint32_t have = reach(cand);
+        if (have >= want) edge = cand;
+        all = have == want;
+    }
+    const int limit = all ? 0x7fffffff : (int)(want - (edge == ~0ull ? 0u : reach(edge + 1)));  // how many of those at the edge
     int above0 = 0, equal0 = 0;
     if (WAVES > 1) {
         int ab = 0, eq = 0;
 #pragma unroll
         for (int n = 0; n < NPL; ++n) {
-            ab += __popcll(__ballot(key(n) > edge));
-            eq += __popcll(__ballot(key(n) == edge));
+            ab += __popcll(__ballot(key[n] > edge));
+            eq += __popcll(__ballot(key[n] == edge));
         }
         if (lane == 0) above_s[wave] = ab, equal_s[wave] = eq;
         __syncthreads();
         for (int w = 0; w < wave; ++w) above0 += above_s[w], equal0 += equal_s[w];
     }
-    const int limit = at_edge ? at_edge : 0x7fffffff;
-    int32_t *out = a.out + row * a.topk;
 #pragma unroll
     for (int n = 0; n < NPL; ++n) {
-        const uint64_t ab = __ballot(key(n) > edge), eq = __ballot(key(n) == edge);
+        const uint64_t ab = __ballot(key[n] > edge), eq = __ballot(key[n] == edge);
         const int rank = equal0 + __popcll(eq & below);
-        const bool take = key(n) > edge || (key(n) == edge && rank < limit);
+        const bool take = key[n] > edge || (key[n] == edge && rank < limit);
         if (take) out[above0 + __popcll(ab & below) + min(rank, limit)] = j0 + 64 * n;
         above0 += __popcll(ab);
         equal0 += __popcll(eq);
     }
-    for (int i = count + (WAVES == 1 ? lane : (int)threadIdx.x); i < a.topk; i += WAVES == 1 ? 64 : WAVES * 64) out[i] = -1;
 }
 
 template <int WAVES, int NPL> int launch_topk(const TopkArgs &a, hipStream_t st) {
