@@ -20,6 +20,7 @@ struct BlockAttnArgs {
     float *delta;              // [B, H, Sq]: rowsum(dout * o) - dlse
     const int32_t *blocks;     // [B, Hk, nQ, topk]
     const int32_t *klen, *qlen;  // [B] or NULL
+    u32x4 *stat;               // backward: [B, H, nQ * bq] a row's lse and delta as parts (block_attn_bwd.hip)
     int32_t *cnt;              // backward: [B, Hk, nK, nQ] how often query block i names key block j
     float *part_o, *part_ml;   // split form: unnormalised partial results, (reference, sum) pairs
     int B, H, Hk, G, Sq, Sk, D, nQ, nK, topk, bq, bk, nsplit;

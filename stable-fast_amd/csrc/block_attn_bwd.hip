@@ -6,8 +6,7 @@
 //   * two kernels instead of atomics, so that the same call gives the same bits: one streams the listed key blocks past a query block (dQ),
 //     one streams the query blocks past a key block (dK, dV).
 //   * the second needs the lists the other way round: a small kernel counts, per key block, how often each query block names it (integer
-//     atomics: their order changes nothing), and the workgroup of a key block walks its row of counts. A count m enters as
-//     2^(s - lse + log2 m).
+//     atomics: their order changes nothing), and the workgroup of a key block walks its row of counts.
 //   * both keep their own rows' operands and sums in registers and read the streamed tiles from LDS as rows (scores, dP) and transposed (sums).
 #include "block_attn.h"
 
@@ -19,16 +18,36 @@ constexpr int BB_LIST = 1024, BB_NAMES = 256;  // list entries, query blocks hel
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 16; }
-template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + BB_NAMES * 2 * 4 + 2 * 2 * 64 * 4 + 16; }
+template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + 2 * 1024 + BB_NAMES * 2 * 4 + 16; }
 
-// delta of a row: 16 lanes, 8 elements each
-template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a) {
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, s, h)
+// What a row's statistics enter the dkv kernel's products as: -lse / scale and -delta, each as four numbers of the type times fixed powers of
+// two (one more matrix instruction starts the accumulators from their sums). Together they hold 32 bits and more; parts below the type's
+// normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied.
+constexpr float BB_PART[4] = {32768.f, 16.f, 1.f / 128.f, 1.f / 16384.f};
+template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
+    typename Elem<T>::vec4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x * (1.f / BB_PART[i]);
+        if (fabsf(a) < 6.103515625e-5f) a = 0.f;
+        v[i] = Elem<T>::from_f32(a);
+        const float taken = (float)v[i];
+        x = taken != taken || fabsf(taken) == INFINITY ? 0.f : fmaf(-taken, BB_PART[i], x);
+    }
+    return __builtin_bit_cast(u32x2, v);
+}
+
+// A row's delta (16 lanes, 8 elements each) and parts; rows up to whole query blocks exist and are marked empty. Clears the counts as well.
+template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a, int64_t rows, int64_t cells) {
+    const int64_t at0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t i = at0; i < cells; i += (int64_t)gridDim.x * 256) a.cnt[i] = 0;
+    const int64_t row = at0 >> 4;  // (b, s, h)
     const int d = (threadIdx.x & 15) * 8;
-    if (row >= (int64_t)a.B * a.Sq * a.H) return;
+    if (row >= rows) return;
+    const int Sp = a.nQ * a.bq;
     const int h = (int)(row % a.H);
     const int64_t bs = row / a.H;
-    const int s = (int)(bs % a.Sq), b = (int)(bs / a.Sq);
+    const int s = (int)(bs % Sp), b = (int)(bs / Sp);
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
     float sum = 0.f;
     if (s < qlen && d < a.D) {
@@ -46,14 +65,17 @@ template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_ke
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
     if (d == 0) {
-        const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
-        if (a.dlse && s < qlen) sum -= a.dlse[at];
-        a.delta[at] = sum;
+        float L = -INFINITY;
+        if (s < a.Sq) {
+            const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
+            if (a.dlse && s < qlen) sum -= a.dlse[at];
+            a.delta[at] = sum;
+            if (s < qlen) L = a.lse[at];
+        }
+        // a row without keys: probabilities 0
+        const u32x2 x = bb_parts<T>(L == -INFINITY ? -INFINITY : -L / a.scale), y = bb_parts<T>(-sum);
+        a.stat[((int64_t)b * a.H + h) * Sp + s] = u32x4{x[0], x[1], y[0], y[1]};
     }
-}
-
-__global__ void __launch_bounds__(256) block_attn_zero_kernel(int32_t *p, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
 
 // cnt[pair][key block][query block] += 1 for every entry that names something
@@ -205,9 +227,9 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, NT = NW * 64;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    int *names = reinterpret_cast<int *>(smem + 4 * TILE);       // query block, count of it
-    float *stat = reinterpret_cast<float *>(names + 2 * BB_NAMES);  // two stages of 64 (lse in log2 units - log2 count), 64 delta
-    int *n_p = reinterpret_cast<int *>(stat + 2 * 2 * 64);
+    char *const stat = smem + 4 * TILE;                           // two stages of 64 rows' parts
+    int *names = reinterpret_cast<int *>(stat + 2 * 1024);        // query block, count of it
+    int *n_p = names + 2 * BB_NAMES;
 
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
@@ -236,6 +258,9 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
     BaLoader<DP, NW> ql, gl;
     ql.init(wave, lane, a.qs[1], a.D);
     gl.init(wave, lane, a.dos[1], a.D);
+    vec8 powers;  // B operand of the statistics' parts
+#pragma unroll
+    for (int i = 0; i < 8; ++i) powers[i] = Elem<T>::from_f32(i < 4 && hi == 0 ? BB_PART[i & 3] : 0.f);
     f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -253,16 +278,9 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
         char *Qs = smem + stage * (2 * TILE);
         ql.load((const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)h * a.qs[2], a.qs[1], a.D, s0, qlen - s0, Qs, wave);
         gl.load((const T *)a.dout + (int64_t)b * a.dos[0] + (int64_t)h * a.dos[2], a.dos[1], a.D, s0, qlen - s0, Qs + TILE, wave);
-        if (tid < 64) {
-            float L = INFINITY, dl = 0.f;
-            if (s0 + tid < qlen) {
-                const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s0 + tid;
-                const float v = a.lse[at];
-                if (v != -INFINITY) L = v * LOG2E - __log2f((float)names[2 * e + 1]);
-                dl = a.delta[at];
-            }
-            stat[stage * 128 + tid] = L;
-            stat[stage * 128 + 64 + tid] = dl;
+        if (wave == NW - 1) {
+            const u32x4 *rows = a.stat + ((int64_t)b * a.H + h) * (a.nQ * a.bq) + s0;
+            ba_dma(ba_rsrc(rows, 1024), (ba_lds_t)(stat + stage * 1024), lane * 16);
         }
     };
 
@@ -285,7 +303,8 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
         if (steps > 0) request(0, 0);
         for (int x = 0; x < steps; ++x) {
             const char *Qs = smem + (x & 1) * (2 * TILE), *Gs = Qs + TILE;
-            const float *Ls = stat + (x & 1) * 128;
+            const char *Ls = stat + (x & 1) * 1024;
+            const int count = __builtin_amdgcn_readfirstlane(names[2 * (x / per) + 1]);
             ba_sync();
             if (x + 1 < steps) request(x + 1, (x + 1) & 1);
 #pragma unroll
@@ -297,9 +316,13 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                     gf[kd] = ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi);
                 }
                 __builtin_amdgcn_sched_barrier(0);
+                const u32x4 parts = *reinterpret_cast<const u32x4 *>(Ls + (rb * 32 + l31) * 16);
                 f32x16 sc, dp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+                // s - lse / scale and dP - delta
+                sc = ba_mfma(__builtin_bit_cast(vec8, u32x4{hi ? 0u : parts[0], hi ? 0u : parts[1], 0u, 0u}), powers, sc);
+                dp = ba_mfma(__builtin_bit_cast(vec8, u32x4{hi ? 0u : parts[2], hi ? 0u : parts[3], 0u, 0u}), powers, dp);
 #pragma unroll
                 for (int kd = 0; kd < KD; ++kd) {
                     sc = ba_mfma(qf[kd], kf[kd], sc);
@@ -316,16 +339,11 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                 __builtin_amdgcn_sched_barrier(0);
                 vec8 p8[2], ds[2];
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    const f32x4 L = *reinterpret_cast<const f32x4 *>(Ls + rb * 32 + 8 * q4 + 4 * hi);
-                    const f32x4 dl = *reinterpret_cast<const f32x4 *>(Ls + 64 + rb * 32 + 8 * q4 + 4 * hi);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = 4 * q4 + r;
-                        const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L[r]));
-                        p8[i >> 3][i & 7] = Elem<T>::from_f32(p);
-                        ds[i >> 3][i & 7] = Elem<T>::from_f32(p * (dp[i] - dl[r]));
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    float p = __builtin_amdgcn_exp2f(sc[i] * c);
+                    if (count != 1) p *= (float)count;
+                    p8[i >> 3][i & 7] = Elem<T>::from_f32(p);
+                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * dp[i]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
@@ -374,15 +392,12 @@ template <typename T, int DP> int set_attr() {
 
 template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
     const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ, entries = (int64_t)a.B * a.Hk * a.nQ * a.topk;
-    const int64_t rows = (int64_t)a.B * a.Sq * a.H;
-    hipLaunchKernelGGL(block_attn_zero_kernel, dim3((unsigned)(cells < 1024 * 256 ? ceil_div64(cells, 256) : 1024)), dim3(256), 0, st, a.cnt, cells);
-    int rc = check_launch("block_attention_backward zero");
+    const int64_t rows = (int64_t)a.B * a.nQ * a.bq * a.H;
+    hipLaunchKernelGGL((block_attn_delta_kernel<T>), dim3((unsigned)ceil_div64(rows, 16)), dim3(256), 0, st, a, rows, cells);
+    int rc = check_launch("block_attention_backward delta");
     if (rc) return rc;
     hipLaunchKernelGGL(block_attn_count_kernel, dim3((unsigned)ceil_div64(entries, 256)), dim3(256), 0, st, a, entries);
     rc = check_launch("block_attention_backward count");
-    if (rc) return rc;
-    hipLaunchKernelGGL((block_attn_delta_kernel<T>), dim3((unsigned)ceil_div64(rows, 16)), dim3(256), 0, st, a);
-    rc = check_launch("block_attention_backward delta");
     if (rc) return rc;
     a.nblk = a.B * a.Hk * a.nQ * a.G;
     a.chunk = ceil_div(a.nblk, 8);
@@ -401,6 +416,7 @@ template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
     return check_launch("block_attention_backward dkv");
 }
 
+static int64_t padded_rows(const sfast_block_attn_params *p) { return (int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) * p->block_q; }
 static int64_t delta_floats(const sfast_block_attn_params *p) { return ((int64_t)p->B * p->H * p->Sq + 3) / 4 * 4; }
 static int64_t cells(const sfast_block_attn_params *p) {
     return (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) * ceil_div(p->Sq, p->block_q);
@@ -422,7 +438,7 @@ using namespace sfast;
 
 extern "C" size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p) {
     if (block_attn_check(p) != SFAST_OK) return 0;
-    return (size_t)(delta_floats(p) + cells(p)) * 4;
+    return (size_t)padded_rows(p) * 16 + (size_t)(delta_floats(p) + cells(p)) * 4;
 }
 
 extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
@@ -442,14 +458,15 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     }
     SFAST_REQUIRE(p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: row stride too long");
     SFAST_REQUIRE((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) <= (1ll << 30) && (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) <= (1ll << 30) &&
-                      (int64_t)p->B * p->Sq * p->H <= (1ll << 34) && (int64_t)p->B * p->Hk * ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 38),
+                      padded_rows(p) <= (1ll << 34) && (int64_t)p->B * p->Hk * ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 38),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_attention_backward: workspace too small");
     BlockAttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.o = out, a.o_rest = out_rest, a.dout = dout, a.lse = const_cast<float *>(lse), a.dlse = dlse, a.dq = dq, a.dk = dk, a.dv = dv;
     a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths;
-    a.delta = (float *)workspace;
+    a.stat = (u32x4 *)workspace;
+    a.delta = (float *)(a.stat + padded_rows(p));
     a.cnt = (int32_t *)(a.delta + delta_floats(p));
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
     a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
