@@ -37,56 +37,58 @@ template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
     return __builtin_bit_cast(u32x2, v);
 }
 
-// A row's delta (16 lanes, 8 elements each) and parts; rows up to whole query blocks exist and are marked empty. Clears the counts as well.
-template <typename T> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a, int64_t rows, int64_t cells) {
-    const int64_t at0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (int64_t i = at0; i < cells; i += (int64_t)gridDim.x * 256) a.cnt[i] = 0;
-    const int64_t row = at0 >> 4;  // (b, s, h)
-    const int d = (threadIdx.x & 15) * 8;
-    if (row >= rows) return;
+// A row's delta (LPR lanes, 8 elements each) and parts; rows up to whole query blocks exist and are marked empty. Clears the counts as well.
+// Bound by reading out, what its rounding left, and its gradient once.
+template <typename T, int LPR> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a, int64_t cells) {
+    const int64_t blocks = (int64_t)gridDim.x * gridDim.y;
+    for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < cells; i += blocks * 256) a.cnt[i] = 0;
+    const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;  // (s, h) of sequence b
+    const int d = (threadIdx.x % LPR) * 8, b = blockIdx.y;
     const int Sp = a.nQ * a.bq;
-    const int h = (int)(row % a.H);
-    const int64_t bs = row / a.H;
-    const int s = (int)(bs % Sp), b = (int)(bs / Sp);
+    if (row >= (uint32_t)Sp * (uint32_t)a.H) return;
+    const int s = (int)(row / (uint32_t)a.H), h = (int)(row - (uint32_t)s * (uint32_t)a.H);
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
     float sum = 0.f;
     if (s < qlen && d < a.D) {
-        float x[8], y[8];
-        unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.dout + b * a.dos[0] + s * a.dos[1] + h * a.dos[2] + d), x);
-        unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.o + b * a.os[0] + s * a.os[1] + h * a.os[2] + d), y);
+        const int64_t at = b * a.os[0] + s * a.os[1] + h * a.os[2] + d;
+        const u32x4 g = *reinterpret_cast<const u32x4 *>((const T *)a.dout + b * a.dos[0] + s * a.dos[1] + h * a.dos[2] + d);
+        const u32x4 o = *reinterpret_cast<const u32x4 *>((const T *)a.o + at);
+        u32x4 z = {0u, 0u, 0u, 0u};
+        if (a.o_rest) z = *reinterpret_cast<const u32x4 *>((const T *)a.o_rest + at);  // out to 16 more bits: in a row that attends to few keys dP - delta cancels
+        float x[8], y[8], w[8];
+        unpack8<T>(g, x);
+        unpack8<T>(o, y);
+        unpack8<T>(z, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
-        if (a.o_rest) {  // out to 16 more bits: in a row that attends to few keys dP - delta cancels
-            unpack8<T>(*reinterpret_cast<const u32x4 *>((const T *)a.o_rest + b * a.os[0] + s * a.os[1] + h * a.os[2] + d), y);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], y[i], sum);
-        }
+        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], w[i], sum);
     }
 #pragma unroll
-    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (d >= 16) return;
+    // the first lane writes lse's parts, the second delta and its parts
+    const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
+    float x;
     if (d == 0) {
-        float L = -INFINITY;
-        if (s < a.Sq) {
-            const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
-            if (a.dlse && s < qlen) sum -= a.dlse[at];
-            a.delta[at] = sum;
-            if (s < qlen) L = a.lse[at];
-        }
-        // a row without keys: probabilities 0
-        const u32x2 x = bb_parts<T>(L == -INFINITY ? -INFINITY : -L / a.scale), y = bb_parts<T>(-sum);
-        a.stat[((int64_t)b * a.H + h) * Sp + s] = u32x4{x[0], x[1], y[0], y[1]};
+        const float L = s < qlen ? a.lse[at] : -INFINITY;
+        x = L == -INFINITY ? -INFINITY : -L / a.scale;  // a row without keys: probabilities 0
+    } else {
+        if (a.dlse && s < qlen) sum -= a.dlse[at];
+        if (s < a.Sq) a.delta[at] = sum;
+        x = -sum;
     }
+    reinterpret_cast<u32x2 *>(a.stat + ((int64_t)b * a.H + h) * Sp + s)[d == 0 ? 0 : 1] = bb_parts<T>(x);
 }
 
 // cnt[pair][key block][query block] += 1 for every entry that names something
-__global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnArgs a, int64_t entries) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= entries) return;
-    const int64_t list = e / a.topk, pair = list / a.nQ;
-    const int qb = (int)(list - pair * a.nQ), b = (int)(pair / a.Hk);
+__global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnArgs a) {
+    const int e = blockIdx.x * 256 + threadIdx.x;  // entry of the lists of one (batch, key head)
+    if (e >= a.nQ * a.topk) return;
+    const int pair = blockIdx.y, qb = e / a.topk, b = pair / a.Hk;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
-    const int j = a.blocks[e];
-    if (j >= 0 && (int64_t)j * a.bk < klen) atomicAdd(a.cnt + (pair * a.nK + j) * a.nQ + qb, 1);
+    const int j = a.blocks[(int64_t)pair * a.nQ * a.topk + e];
+    if (j >= 0 && (int64_t)j * a.bk < klen) atomicAdd(a.cnt + ((int64_t)pair * a.nK + j) * a.nQ + qb, 1);
 }
 
 // dQ of one query block: the forward's streams, K read as rows (scores) and transposed (dQ), V as rows (dP)
@@ -391,12 +393,15 @@ template <typename T, int DP> int set_attr() {
 }
 
 template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
-    const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ, entries = (int64_t)a.B * a.Hk * a.nQ * a.topk;
-    const int64_t rows = (int64_t)a.B * a.nQ * a.bq * a.H;
-    hipLaunchKernelGGL((block_attn_delta_kernel<T>), dim3((unsigned)ceil_div64(rows, 16)), dim3(256), 0, st, a, rows, cells);
+    const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ;
+    const int64_t rows = (int64_t)a.nQ * a.bq * a.H;
+    if (DP == 64)
+        hipLaunchKernelGGL((block_attn_delta_kernel<T, 8>), dim3((unsigned)ceil_div64(rows, 32), a.B), dim3(256), 0, st, a, cells);
+    else
+        hipLaunchKernelGGL((block_attn_delta_kernel<T, 16>), dim3((unsigned)ceil_div64(rows, 16), a.B), dim3(256), 0, st, a, cells);
     int rc = check_launch("block_attention_backward delta");
     if (rc) return rc;
-    hipLaunchKernelGGL(block_attn_count_kernel, dim3((unsigned)ceil_div64(entries, 256)), dim3(256), 0, st, a, entries);
+    hipLaunchKernelGGL(block_attn_count_kernel, dim3((unsigned)ceil_div(a.nQ * a.topk, 256), a.B * a.Hk), dim3(256), 0, st, a);
     rc = check_launch("block_attention_backward count");
     if (rc) return rc;
     a.nblk = a.B * a.Hk * a.nQ * a.G;
@@ -458,7 +463,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     }
     SFAST_REQUIRE(p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: row stride too long");
     SFAST_REQUIRE((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) <= (1ll << 30) && (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) <= (1ll << 30) &&
-                      padded_rows(p) <= (1ll << 34) && (int64_t)p->B * p->Hk * ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 38),
+                      padded_rows(p) / p->B <= (1ll << 30) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_attention_backward: workspace too small");
