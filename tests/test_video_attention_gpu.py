@@ -553,6 +553,87 @@ def test_captured_calls_replay_on_new_inputs(Sq):
     del g1, g2
 
 
+def test_a_captured_training_step():
+    """Forward and gradients in one graph (no eager graph of the same leaves is alive: that is what torch asks of any captured backward)."""
+    case = (1, 200, 300, 4, 2, 64, 128, 64, 3, None, None)
+    q, k, v, blocks = make(case, BF16, 1)
+    pos = torch.arange(300, device="cuda")[:, None].repeat(1, 3)
+    go = randn(q.shape, BF16, 9)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def step():
+        kr = OPS.rotary_embedding_nd(leaves[1], None, pos, [16, 24, 24])[0]
+        out, lse = ATT.block_sparse_attention(leaves[0], kr, leaves[2], blocks)
+        return (out.detach(), lse.detach()) + torch.autograd.grad(out, leaves, go)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (5, 6, 7):
+        with torch.no_grad():
+            for i, t in enumerate(leaves):
+                t.copy_(randn(t.shape, BF16, 10 * seed + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        got_now = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(got_now, step()))
+    del graph
+
+
+def test_a_nan_key_reaches_the_rows_that_name_it_only():
+    case = (1, 300, 500, 2, 2, 64, 64, 64, 2, None, None)
+    q, k, v, blocks = make(case, F16, 4)
+    want = R.attention(q, k, v, blocks, 64, 64)["out"]
+    for bad in (math.nan, math.inf):
+        kk = k.clone()
+        kk[0, 70, 1, 3] = bad                         # block 1 of the second head
+        out, lse = ATT.block_sparse_attention(q, kk, v, blocks, 64, 64)
+        names = (blocks[0, 1] == 1).any(-1).repeat_interleave(64)[:300]
+        clean = torch.ones((300, 2), dtype=torch.bool, device="cuda")
+        clean[:, 1] = ~names
+        assert names.any() and not names.all()
+        assert torch.isfinite(out[0][clean]).all()
+        if math.isnan(bad):
+            assert torch.isnan(out[0, :, 1][names]).all()
+        else:                                          # a score of +inf leaves no number, one of -inf takes the key out
+            up = names & (q[0, :, 1, 3] > 0)
+            down = names & (q[0, :, 1, 3] < 0)
+            assert torch.isnan(out[0, :, 1][up]).all() and torch.isfinite(out[0, :, 1][down]).all()
+        off = (out.double() - want[0]).abs() > want[1]
+        assert not off[0][clean].any()
+
+
+def test_batch_invariant_mode_cuts_lists_alike_for_every_batch(monkeypatch):
+    """SFAST_BATCH_INVARIANT=1: a sample's bits do not depend on how many ride with it (the parts of its lists are those of the reference batch)."""
+    from sfast.hip import lib as L
+    lib = L.load()
+    B, Sq, Sk, H, Hk, D = 24, 1, 4000, 8, 2, 128
+    q, k, v, blocks = make((B, Sq, Sk, H, Hk, D, 128, 64, 40, None, None), BF16, 2)
+
+    def rows(n):
+        return ATT.block_sparse_attention(q[:n], k[:n], v[:n], blocks[:n])
+    monkeypatch.setenv("SFAST_BATCH_INVARIANT", "1")
+    try:
+        assert lib.sfast_hip_init() == 0
+        a, b, c = rows(1), rows(2), rows(B)
+        for x, y in ((a, b), (a, c), (b, c)):
+            n = min(len(x[0]), len(y[0]))
+            assert torch.equal(x[0][:n], y[0][:n]) and torch.equal(x[1][:n], y[1][:n])
+    finally:
+        monkeypatch.undo()
+        assert lib.sfast_hip_init() == 0
+    want = R.attention(q, k, v, blocks, 128, 64)
+    R.check("out", c[0], *want["out"])
+    R.check("out", rows(B)[0], *want["out"])
+
+
 def test_two_streams_at_once():
     case = (1, 300, 600, 4, 2, 64, 128, 64, 4, None, None)
     ins = [make(case, BF16, s) for s in (1, 100)]
