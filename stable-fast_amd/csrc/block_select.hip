@@ -80,7 +80,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 struct TopkArgs {
     const float *qm, *km;
     const int32_t *klen;
-    double *score;    // [B, Hk, nQ, nK]
+    uint32_t *high, *low;  // [B, Hk, nQ, nK]: the halves of the scores' keys
     int32_t *out;     // [B, Hk, nQ, topk]
     int B, nQ, nK, H, Hk, G, D, topk, bk;
 };
@@ -89,6 +89,21 @@ __device__ __forceinline__ int topk_count(const TopkArgs &a, int b) {
     if (!a.klen) return a.nK;
     const uint32_t n = ((uint32_t)max(a.klen[b], 0) + (uint32_t)(a.bk - 1)) / (uint32_t)a.bk;
     return (int)min(n, (uint32_t)a.nK);
+}
+
+// a score as a 64-bit key whose order is the score's (NaN above all, -0 and 0 alike, 0 is no key)
+__device__ __forceinline__ uint64_t topk_key(double s) {
+    s += 0.0;  // -0 and 0 are one score
+    const uint64_t u = __builtin_bit_cast(uint64_t, s);
+    if (s != s) return ~0ull;
+    return (u >> 63) ? ~u : (u | (1ull << 63));
+}
+
+// the upper halves decide nearly always: they are kept apart, and the lower ones are read only where they do not
+__device__ __forceinline__ void put_key(const TopkArgs &a, int64_t at, double s) {
+    const uint64_t k = topk_key(s);
+    a.high[at] = (uint32_t)(k >> 32);
+    a.low[at] = (uint32_t)k;
 }
 
 template <int MI, int NJ> __global__ void __launch_bounds__(256, 4) block_score_kernel(const TopkArgs a) {
@@ -155,11 +170,11 @@ template <int MI, int NJ> __global__ void __launch_bounds__(256, 4) block_score_
         for (int r = 0; r < 4; ++r) {
             const int i = i0 + 16 * x + 4 * r + l4;
             if (i >= a.nQ) continue;
-            double *row = a.score + ((int64_t)pair * a.nQ + i) * a.nK;
+            const int64_t row = ((int64_t)pair * a.nQ + i) * a.nK;
 #pragma unroll
             for (int y = 0; y < NJ; ++y) {
                 const int j = j0 + 16 * y + l15;
-                if (j < count) row[j] = acc[x][y][r];
+                if (j < count) put_key(a, row + j, acc[x][y][r]);
             }
         }
 }
@@ -207,13 +222,13 @@ __global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) 
                 }
             }
         }
-        double *row = a.score + ((int64_t)pair * a.nQ + i) * a.nK;
+        const int64_t row = ((int64_t)pair * a.nQ + i) * a.nK;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
 #pragma unroll
             for (int off = 4; off >= 1; off >>= 1) s[y] += __shfl_xor(s[y], off, 64);
             const int j = j0 + 8 * y + l8;
-            if (l7 == 0 && j < count) row[j] = s[y];
+            if (l7 == 0 && j < count) put_key(a, row + j, s[y]);
         }
     }
 }
@@ -223,13 +238,6 @@ __global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) 
 // the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. It starts below the
 // bits that all keys share and looks at the upper 31 bits first: those settle all but near-ties, for two instructions a key and bit (a
 // comparison's mask would cost wait states on top). Keys equal to the threshold are taken in the order of their index.
-__device__ __forceinline__ uint64_t topk_key(double s) {
-    s += 0.0;  // -0 and 0 are one score
-    const uint64_t u = __builtin_bit_cast(uint64_t, s);
-    if (s != s) return ~0ull;
-    return (u >> 63) ? ~u : (u | (1ull << 63));
-}
-
 // sum / maximum over a wave, the same in every lane (row shifts by 1, 2, 4, 8, then across the rows of 16: lane 63 holds the result)
 template <int CTRL> __device__ __forceinline__ uint32_t topk_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
@@ -237,6 +245,11 @@ template <int CTRL> __device__ __forceinline__ uint32_t topk_dpp(uint32_t v) {
 __device__ __forceinline__ uint32_t topk_wave_sum(uint32_t v) {
     v += topk_dpp<0x111>(v), v += topk_dpp<0x112>(v), v += topk_dpp<0x114>(v), v += topk_dpp<0x118>(v);
     v += topk_dpp<0x142>(v), v += topk_dpp<0x143>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t topk_wave_or(uint32_t v) {
+    v |= topk_dpp<0x111>(v), v |= topk_dpp<0x112>(v), v |= topk_dpp<0x114>(v), v |= topk_dpp<0x118>(v);
+    v |= topk_dpp<0x142>(v), v |= topk_dpp<0x143>(v);
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ uint32_t topk_wave_max(uint32_t v) {
@@ -254,25 +267,20 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
     const int64_t row = row_id;
     const int count = topk_count(a, row_id / a.nQ / a.Hk);
     const int j0 = wave * 64 * NPL + lane;
-    uint64_t key[NPL];
-    uint32_t up[NPL];  // the upper 31 bits
-    double score[NPL];
+    uint32_t up[NPL];  // the upper 31 bits of the keys
 #pragma unroll
-    for (int n = 0; n < NPL; ++n) score[n] = a.score[row * a.nK + min(j0 + 64 * n, a.nK - 1)];  // all in flight, whether they count or not
+    for (int n = 0; n < NPL; ++n) up[n] = a.high[row * a.nK + min(j0 + 64 * n, a.nK - 1)];  // all in flight, whether they count or not
 #pragma unroll
-    for (int n = 0; n < NPL; ++n) {
-        key[n] = j0 + 64 * n < count ? topk_key(score[n]) : 0ull;
-        up[n] = (uint32_t)(key[n] >> 33);
-    }
+    for (int n = 0; n < NPL; ++n) up[n] = j0 + 64 * n < count ? up[n] >> 1 : 0u;
     int turn = 0;
-    const auto over_waves = [&](uint32_t mine, bool most) __attribute__((always_inline)) -> uint32_t {
+    const auto over_waves = [&](uint32_t mine, bool most, bool any = false) __attribute__((always_inline)) -> uint32_t {
         if (WAVES == 1) return mine;
         turn ^= 1;
         if (lane == 0) sums[turn][wave] = mine;
         __syncthreads();
         uint32_t s = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) s = most ? max(s, sums[turn][w]) : s + sums[turn][w];
+        for (int w = 0; w < WAVES; ++w) s = any ? s | sums[turn][w] : most ? max(s, sums[turn][w]) : s + sums[turn][w];
         return s;
     };
     int32_t *out = a.out + row * a.topk;
@@ -329,17 +337,36 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
         }
         return;
     }
-    // Scores that agree in their upper 31 bits stand at the border: the topk-th key has the upper bits edge_up; the other 33 decide, then the index.
+    // Scores that agree in their upper 31 bits stand at the border: the topk-th key has the upper bits edge_up, the other 33 decide, then the
+    // index. The keys are read again as they are needed, and the search starts below the bits that the ones at the border share (equal scores
+    // need none).
     const uint32_t want = (uint32_t)a.topk;
-    uint64_t edge = (uint64_t)edge_up << 33;
+    const auto key = [&](int n) __attribute__((always_inline)) -> uint64_t {
+        const int64_t at = row * a.nK + min(j0 + 64 * n, a.nK - 1);
+        return j0 + 64 * n < count ? ((uint64_t)a.high[at] << 32) | a.low[at] : 0ull;
+    };
     const auto reach = [&](uint64_t from) __attribute__((always_inline)) -> uint32_t {
         uint32_t mine = 0;
-#pragma unroll
-        for (int n = 0; n < NPL; ++n) mine += key[n] >= from ? 1u : 0u;
+#pragma unroll 4
+        for (int n = 0; n < NPL; ++n) mine += key(n) >= from ? 1u : 0u;
         return over_waves(topk_wave_sum(mine), false);
     };
+    uint32_t share_hi = 0, share_lo = 0, miss_hi = 0, miss_lo = 0;
+#pragma unroll 4
+    for (int n = 0; n < NPL; ++n) {
+        const uint64_t k = key(n);
+        if ((uint32_t)(k >> 33) == edge_up && k != 0) {
+            share_hi |= (uint32_t)(k >> 32), share_lo |= (uint32_t)k;       // bits that some key has
+            miss_hi |= ~(uint32_t)(k >> 32), miss_lo |= ~(uint32_t)k;       // bits that some key lacks
+        }
+    }
+    share_hi = over_waves(topk_wave_or(share_hi), true, true), share_lo = over_waves(topk_wave_or(share_lo), true, true);
+    miss_hi = over_waves(topk_wave_or(miss_hi), true, true), miss_lo = over_waves(topk_wave_or(miss_lo), true, true);
+    const uint64_t shared = ((uint64_t)share_hi << 32) | share_lo, differ = shared & (((uint64_t)miss_hi << 32) | miss_lo);
+    const int top = differ ? 63 - __builtin_clzll(differ) : -1;  // below 33
+    uint64_t edge = top < 0 ? shared : shared & ~((2ull << top) - 1ull);
     bool all = false;  // exactly topk keys reach the edge
-    for (int bit = 32; bit >= 0 && !all; --bit) {
+    for (int bit = top; bit >= 0 && !all; --bit) {
         const uint64_t cand = edge | (1ull << bit);
         const uint32_t have = reach(cand);
         if (have >= want) edge = cand;
@@ -349,20 +376,21 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
     int above0 = 0, equal0 = 0;
     if (WAVES > 1) {
         int ab = 0, eq = 0;
-#pragma unroll
+#pragma unroll 4
         for (int n = 0; n < NPL; ++n) {
-            ab += __popcll(__ballot(key[n] > edge));
-            eq += __popcll(__ballot(key[n] == edge));
+            const uint64_t k = key(n);
+            ab += __popcll(__ballot(k > edge));
+            eq += __popcll(__ballot(k == edge));
         }
         if (lane == 0) above_s[wave] = ab, equal_s[wave] = eq;
         __syncthreads();
         for (int w = 0; w < wave; ++w) above0 += above_s[w], equal0 += equal_s[w];
     }
-#pragma unroll
+#pragma unroll 4
     for (int n = 0; n < NPL; ++n) {
-        const uint64_t ab = __ballot(key[n] > edge), eq = __ballot(key[n] == edge);
+        const uint64_t k = key(n), ab = __ballot(k > edge), eq = __ballot(k == edge);
         const int rank = equal0 + __popcll(eq & below);
-        const bool take = key[n] > edge || (key[n] == edge && rank < limit);
+        const bool take = k > edge || (k == edge && rank < limit);
         if (take) out[above0 + __popcll(ab & below) + min(rank, limit)] = j0 + 64 * n;
         above0 += __popcll(ab);
         equal0 += __popcll(eq);
@@ -444,7 +472,8 @@ extern "C" int sfast_hip_block_topk(const float *qm, const float *km, const int3
     SFAST_REQUIRE(workspace && aligned8(workspace) && workspace_bytes >= sfast_hip_block_topk_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_topk: workspace too small");
     TopkArgs a{};
-    a.qm = qm, a.km = km, a.klen = key_lengths, a.out = out, a.score = (double *)workspace;
+    a.qm = qm, a.km = km, a.klen = key_lengths, a.out = out, a.high = (uint32_t *)workspace;
+    a.low = a.high + (size_t)p->B * p->Hk * p->nQ * p->nK;
     a.B = p->B, a.nQ = p->nQ, a.nK = p->nK, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.D = p->D, a.topk = p->topk, a.bk = p->block_k;
     hipStream_t st = (hipStream_t)stream;
     const unsigned pairs = (unsigned)(p->B * p->Hk);
@@ -459,7 +488,9 @@ extern "C" int sfast_hip_block_topk(const float *qm, const float *km, const int3
     rc = check_launch("block_score");
     if (rc) return rc;
     set_kernel_name("block_topk[nK=%d]", p->nK);
-    // a row's keys stay in registers: one wave up to 2048 of them, sixteen waves beyond
+    // a row's keys stay in registers: one wave up to 2048 of them (four from 1025 on where rows are few: 23.8 against 25.9 us for 64 rows of
+    // 2048, but 43.9 against 37.1 for 4500 of 900), sixteen waves beyond
+    if (p->nK > 1024 && p->nK <= 2048 && (int64_t)pairs * p->nQ <= 512) return launch_topk<4, 8>(a, st);
     if (p->nK <= 256) return launch_topk<1, 4>(a, st);
     if (p->nK <= 1024) return launch_topk<1, 16>(a, st);
     if (p->nK <= 2048) return launch_topk<1, 32>(a, st);

@@ -175,6 +175,14 @@ def test_block_topk_ties_zeros_nan_and_infinities():
     assert choose([5.0, nan, 6.0], 2) == [1, 2]
     for values in ([1e-300, 2e-300, 0.0], [2.0, 2.0 + 2.0 ** -22, 2.0]):
         assert choose(values, 1) == [max(range(3), key=lambda i: torch.tensor(values[i]).item())]
+    # scores alike in their upper bits: 2^-22 apart in a product of two fp32 numbers, in every width of the search
+    for n in (40, 200, 1000, 2000, 2049, 9000):
+        qm2 = torch.full((1, 1, 1, 8), 1.0 + 2.0 ** -12, device="cuda")
+        km = torch.full((1, n, 1, 8), 1.0, device="cuda")
+        gen = torch.Generator().manual_seed(n)
+        km[0, :, 0, 0] += (torch.randint(0, 4, (n,), generator=gen) * 2.0 ** -23).cuda()
+        for k in (1, 7, n // 2):
+            assert torch.equal(ATT.block_topk(qm2, km, k).cpu(), R.topk(qm2, km, k, 64))
     big = torch.zeros((1, 3000, 1, 8), device="cuda")          # sixteen waves, all alike, ties over the waves' borders
     assert ATT.block_topk(qm, big, 2500).flatten().tolist() == list(range(2500))
 
