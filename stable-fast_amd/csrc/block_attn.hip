@@ -19,12 +19,15 @@ constexpr int BA_MAX_LIST = 1024;  // entries of one workgroup's (part of a) lis
 
 template <int DP, int NS> constexpr int ba_fwd_lds() { return NS * 2 * BaTile<DP>::BYTES + BA_MAX_LIST * 2 * 4 + 16; }
 
-// NS: LDS stages, NS - 1 tiles are on their way while one is used.
+// NS: LDS stages, NS - 1 tiles are on their way while one is used. KW = 2: two waves share the rows and take a half of every tile's keys each
+// (joined through LDS at the end): where compute units are not full, a tile's chain of products, softmax and products is what takes time.
 // PACK: rows are (query, head of the group) pairs, row = s * G + g, one unit per key head; else one unit per query head.
-template <typename T, int DP, int NW, int NS, bool PACK>
-__global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockAttnArgs a) {
+constexpr int ba_key_waves(int NS, bool PACK) { return PACK || NS > 2 ? 2 : 1; }
+
+template <typename T, int DP, int NW, int NS, bool PACK, int KW = ba_key_waves(NS, PACK)>
+__global__ void __launch_bounds__(NW * KW * 64, 2) block_attn_fwd_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
-    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
+    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, KBN = 2 / KW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     int *tiles = reinterpret_cast<int *>(smem + NS * 2 * TILE);
     int *ntiles_p = tiles + 2 * BA_MAX_LIST;
@@ -41,7 +44,8 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
 
-    const int r = wave * 32 + l31;
+    const int half = KW == 1 ? 0 : wave / NW;  // the half of the keys
+    const int r = (KW == 1 ? wave : wave % NW) * 32 + l31;
     const int s = PACK ? r / a.G : qb * a.bq + r;
     const int h = hk * a.G + (PACK ? r - s * a.G : g0);
     const bool inside = PACK ? s < a.Sq : (r < a.bq && s < a.Sq);  // a row of the output
@@ -69,7 +73,7 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
 
     const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
-    BaLoader<DP, NW> kl, vl;
+    BaLoader<DP, NW * KW> kl, vl;
     kl.init(wave, lane, a.ks[1], a.D);
     vl.init(wave, lane, a.vs[1], a.D);
 
@@ -97,45 +101,45 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
         char *Ks = smem + (t % NS) * (2 * TILE), *Vs = Ks + TILE;
         // tile t has landed (NS - 2 later ones may be on their way), every wave is done with the stage that is requested next
         if (NS > 2 && t + NS - 2 < n)
-            ba_sync<(NS - 2) * 2 * BaLoader<DP, NW>::N>();
+            ba_sync<(NS - 2) * 2 * BaLoader<DP, NW * KW>::N>();
         else
             ba_sync();
         if (t + NS - 1 < n) request(t + NS - 1);
         // scores: all K fragments are requested before the first product (the two key halves alternate: independent accumulators)
-        vec8 kf[2][KD];
+        vec8 kf[KBN][KD];
 #pragma unroll
         for (int kd = 0; kd < KD; ++kd)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) kf[kb][kd] = ba_row_frag<T, DP>(Ks, kb * 32 + l31, kd, hi);
+            for (int kb = 0; kb < KBN; ++kb) kf[kb][kd] = ba_row_frag<T, DP>(Ks, (half + kb) * 32 + l31, kd, hi);
         __builtin_amdgcn_sched_barrier(0);
-        f32x16 sc[2];
+        f32x16 sc[KBN];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KBN; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
 #pragma unroll
         for (int kd = 0; kd < KD; ++kd)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) sc[kb] = ba_mfma(kf[kb][kd], qf[kd], sc[kb]);
+            for (int kb = 0; kb < KBN; ++kb) sc[kb] = ba_mfma(kf[kb][kd], qf[kd], sc[kb]);
         __builtin_amdgcn_sched_barrier(0);
         // V^T fragments of the first half of the keys arrive under the softmax
-        vec8 vf[4][DB];
+        vec8 vf[2 * KBN][DB];
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < KBN; ++g)
 #pragma unroll
-            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, g * 16);
+            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, half * 32 + g * 16);
         __builtin_amdgcn_sched_barrier(0);
         const int left = klen - cur * 64;
         if (left < 64) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < KBN; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hi >= left) sc[kb][i] = -INFINITY;
+                    if ((half + kb) * 32 + (i & 3) + 8 * (i >> 2) + 4 * hi >= left) sc[kb][i] = -INFINITY;
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KBN; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
         mx = ba_xor32_max(mx) * c;
@@ -152,9 +156,9 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
                 for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
         }
         const float ref = m == -INFINITY ? 0.f : m;  // a row whose scores are all -inf keeps the sum 0
-        vec8 p[4];
+        vec8 p[2 * KBN];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KBN; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], c, -ref));
@@ -163,15 +167,37 @@ __global__ void __launch_bounds__(NW * 64, 2) block_attn_fwd_kernel(const BlockA
             }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 2; g < 4; ++g)
+        for (int g = KBN; g < 2 * KBN; ++g)
 #pragma unroll
-            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, g * 16);
+            for (int db = 0; db < DB; ++db) vf[g][db] = ba_col_frag<T, DP>(Vs, lane, db, half * 32 + g * 16);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 2 * KBN; ++g)
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[db] = ba_mfma(vf[g][db], p[g], o[db]);
     }
     l = ba_xor32_sum(l);
+    if constexpr (KW == 2) {
+        // the second half's sums come through LDS (the stages are free, the list is no longer needed)
+        __syncthreads();
+        const int rw = wave % NW;
+        float *const so = reinterpret_cast<float *>(smem) + rw * (DB * 16 * 64) + lane, *const sml = reinterpret_cast<float *>(tiles) + rw * 128 + lane;
+        if (half == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) so[(db * 16 + i) * 64] = o[db][i];
+            sml[0] = m, sml[64] = l;
+        }
+        __syncthreads();
+        if (half == 1) return;
+        const float m1 = sml[0], top = fmaxf(m, m1), base = top == -INFINITY ? 0.f : top;
+        const float w0 = __builtin_amdgcn_exp2f(m - base), w1 = __builtin_amdgcn_exp2f(m1 - base);
+        m = top, l = l * w0 + sml[64] * w1;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] = o[db][i] * w0 + so[(db * 16 + i) * 64] * w1;
+    }
     if (!inside) return;
     if (!row_ok) {  // a row behind its sequence: nothing
         m = -INFINITY, l = 0.f;
@@ -302,8 +328,10 @@ struct Plan {
 // How a call is cut into workgroups.
 //  * Packed rows: all query rows of a group fit 64 rows of one or two waves.
 //  * A list is split over workgroups where that is shorter. Measured: a workgroup takes 1.1 us a tile while compute units are free (512
-//    workgroups are two on each); a split adds 4 us for the second launch and the partial results' way through memory at 0.8 bytes / ps.
-//  * deep: four LDS stages instead of two, for grids that leave one workgroup to a compute unit anyway.
+//    workgroups are two on each), 0.8 us with two waves for the keys; a split adds 4 us for the second launch and the partial results' way
+//    through memory at 0.8 bytes / ps.
+//  * deep: four LDS stages instead of two and two waves for the keys, for grids that leave one workgroup to a compute unit anyway
+//    (2 x 6 x 1000 rows against 8 blocks of 64: 11.7 us, with two stages and one wave 14.7).
 static Plan make_plan(const sfast_block_attn_params *p) {
     Plan pl{};
     const int G = p->H / p->Hk;
@@ -319,10 +347,11 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     if (units < 256) {
         const double rows = pl.pack ? (double)p->Sq * G : pl.nw * 32;
         const double part = 2.0 * units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
-        double best = 1.1 * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
+        const auto tile_us = [&](int64_t blocks) { return pl.pack || blocks <= 256 ? 0.8 : 1.1; };
+        double best = tile_us(units * least) * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
         for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * units <= 1024; ++x) {
             const double rounds = (double)ceil_div64(x * units, 512);
-            const double t = 1.1 * (double)ceil_div64(tiles, x) * rounds + 4.0 + part * (double)x;
+            const double t = tile_us(x * units) * (double)ceil_div64(tiles, x) * rounds + 4.0 + part * (double)x;
             if (t < best) best = t, ns = x;
         }
     }
@@ -336,7 +365,8 @@ template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl,
     const dim3 grid((unsigned)(8 * a.chunk));
     const auto go = [&](auto NW, auto NS, auto PACK) {
         constexpr int nw = decltype(NW)::value, ns = decltype(NS)::value;
-        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * 64), (ba_fwd_lds<DP, ns>()), st, a);
+        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * ba_key_waves(ns, decltype(PACK)::value) * 64),
+                           (ba_fwd_lds<DP, ns>()), st, a);
     };
     const auto with = [&](auto NW, auto PACK) {
         if (pl.deep)
