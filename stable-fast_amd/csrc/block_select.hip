@@ -410,7 +410,7 @@ static int check_topk(const sfast_block_topk_params *p) {
                   "block_topk: bad shape");
     SFAST_REQUIRE(p->H % p->Hk == 0, SFAST_ERR_INVALID, "block_topk: %d query heads are no multiple of %d key heads", p->H, p->Hk);
     SFAST_REQUIRE(p->D % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_topk: head dim %d is no multiple of 4", p->D);
-    SFAST_REQUIRE(p->nK <= 32768, SFAST_ERR_UNSUPPORTED, "block_topk: %d key blocks (up to 32768)", p->nK);
+    SFAST_REQUIRE(p->nK <= 32768 && p->topk <= 32768, SFAST_ERR_UNSUPPORTED, "block_topk: %d of %d key blocks (up to 32768)", p->topk, p->nK);
     SFAST_REQUIRE((int64_t)p->B * p->Hk <= 65535 && p->nQ <= (1 << 20) && (int64_t)p->B * p->Hk * p->nQ <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_topk: too many rows");
     return SFAST_OK;
 }

@@ -772,7 +772,7 @@ def block_topk(query_means, key_means, topk, block_k=64, key_lengths=None):
     """The `topk` key blocks of every query block whose means agree best: fp32 [B, nQ, H, D] and [B, nK, Hk, D] -> int32 [B, Hk, nQ, topk].
     The score of a block is the sum of the products over the heads of a group, in 64 bits (the group shares its choice); blocks that begin
     at or behind key_lengths[b] (block_k keys each) do not take part. Ascending, -1 behind the last one; ties take the lowest block, a NaN
-    score ranks above all. nK <= 32768, D % 4 == 0."""
+    score ranks above all. nK and topk up to 32768, D % 4 == 0."""
     L.load_torch_ops()
     return torch.ops.sfast_xformers.block_topk(query_means, key_means, topk, block_k, key_lengths)
 

@@ -115,6 +115,17 @@ def test_rotary_means_and_choice_refuse_before_they_launch(built_lib):
     assert topk(ws=None) == -3 and topk(nb=2 * 2 * 3 * 9 * 8 - 1) == -3
 
 
+def test_the_choice_refuses_lists_longer_than_any_row(built_lib):
+    """(the entries behind the last block are filled with -1 in steps of 32-bit indexes)"""
+    from sfast.hip import lib as L
+    lib = L.load()
+    for topk in (32769, (1 << 31) - 1):
+        p = L.BlockTopkParams(1, 1, 9, 1, 1, 64, topk, 64)
+        assert lib.sfast_hip_block_topk_workspace_bytes(C.byref(p)) == 0
+        assert lib.sfast_hip_block_topk(4096, 4096, None, 4096, C.byref(p), 4096, 1 << 40, None) == -1
+        assert b"block_topk" in lib.sfast_hip_last_error()
+
+
 def test_operators_take_no_cpu_tensors(built_lib):
     import sfast  # noqa: F401
     from sfast.hip import functional as F
