@@ -411,6 +411,8 @@ int block_attn_check(const sfast_block_attn_params *p) {
                       "block_attention: strides must be multiples of 8 elements");
     // offsets inside one 64-row tile have 32 bits, bit 31 marks an element outside
     SFAST_REQUIRE(p->ks[1] < (1 << 23) && p->vs[1] < (1 << 23) && p->qs[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention: row stride too long");
+    // what lies behind a tile's last row is cut off by its address: rows must not overlap
+    SFAST_REQUIRE(p->ks[1] >= p->D && p->vs[1] >= p->D && p->qs[1] >= p->D, SFAST_ERR_UNSUPPORTED, "block_attention: rows overlap");
     return SFAST_OK;
 }
 

@@ -461,7 +461,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
         SFAST_REQUIRE(p->dqs[i] % 4 == 0 && p->dks[i] % 4 == 0 && p->dvs[i] % 4 == 0, SFAST_ERR_UNSUPPORTED,
                       "block_attention_backward: gradient strides must be multiples of 4 elements");
     }
-    SFAST_REQUIRE(p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: row stride too long");
+    SFAST_REQUIRE(p->dos[1] >= p->D && p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: rows overlap, or their stride is too long");
     SFAST_REQUIRE((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) <= (1ll << 30) && (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) <= (1ll << 30) &&
                       padded_rows(p) / p->B <= (1ll << 30) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");

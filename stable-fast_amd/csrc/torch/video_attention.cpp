@@ -286,11 +286,11 @@ struct Attention {
     }
 };
 
-// The kernels read 16-byte runs of a row: head-dim stride 1, other strides multiples of 8, an aligned address, rows less than 2^23 elements
-// apart. Anything else is copied.
+// The kernels read 16-byte runs of a row: head-dim stride 1, other strides multiples of 8, an aligned address, rows that do not overlap and
+// are less than 2^23 elements apart. Anything else is copied.
 Tensor rows16(const Tensor &t) {
     const bool ok = t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && (uintptr_t)t.const_data_ptr() % 16 == 0 &&
-                    t.stride(1) < (1 << 23);
+                    t.stride(1) >= t.size(3) && t.stride(1) < (1 << 23);
     return ok ? t : contiguous_copy(t);
 }
 

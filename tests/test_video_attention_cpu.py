@@ -115,6 +115,18 @@ def test_rotary_means_and_choice_refuse_before_they_launch(built_lib):
     assert topk(ws=None) == -3 and topk(nb=2 * 2 * 3 * 9 * 8 - 1) == -3
 
 
+@pytest.mark.parametrize("name", ["qs", "ks", "vs", "dos"])
+def test_block_attention_refuses_rows_that_overlap(built_lib, name):
+    from sfast.hip import lib as L
+    lib = L.load()
+    p = attn_params(L, **{name: (300 * 64 * 4, 56, 64)})
+    args = [4096, 4096, 4096, 4096, None, None, 4096, 4096, None]
+    if name != "dos":
+        assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, 1 << 40, None) == -1
+    back = [4096, 4096, 4096, 4096, None, None, 4096, None, 4096, 4096, None, 4096, 4096, 4096]
+    assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, 1 << 40, None) == -1
+
+
 def test_the_choice_refuses_lists_longer_than_any_row(built_lib):
     """(the entries behind the last block are filled with -1 in steps of 32-bit indexes)"""
     from sfast.hip import lib as L

@@ -338,6 +338,21 @@ def test_block_attention_strides(dtype, grads):
     attend(case, heads_first, kv[:, :, 0], kv[:, :, 1], wide, grads=grads)
 
 
+def test_block_attention_rows_that_overlap():
+    """Rows that share memory (windows over a line of numbers), the last one with an infinity: it stays in its own column."""
+    D, S = 16, 5
+    gen = torch.Generator().manual_seed(3)
+    lines = [torch.randn(8 * (S - 1) + D, generator=gen).to(F16) for _ in range(3)]
+    lines[2][-1] = float("inf")
+    got = [t.cuda().as_strided((1, S, 1, D), (128, 8, 16, 1)) for t in lines]
+    want = [t.as_strided((1, S, 1, D), (128, 8, 16, 1)).contiguous().cuda() for t in lines]
+    blocks = torch.zeros(1, 1, 1, 1, dtype=torch.int32, device="cuda")
+    out, lse = F.block_sparse_attention(*got, blocks)
+    assert torch.isfinite(out[..., :-1]).all() and torch.isinf(out[..., -1]).all()
+    same, lse2 = F.block_sparse_attention(*want, blocks)
+    assert torch.equal(out, same) and torch.equal(lse, lse2)
+
+
 def test_block_attention_gradient_of_an_expanded_and_of_an_unused_result():
     case = CASES[9]
     B, Sq, Sk, H, Hk, D, bq, bk, topk, kl, ql = case
