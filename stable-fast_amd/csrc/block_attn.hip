@@ -455,7 +455,8 @@ extern "C" int sfast_hip_block_attention(const void *q, const void *k, const voi
     SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out) && aligned8(out_rest), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) SFAST_REQUIRE(p->os[i] % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_attention: output strides must be multiples of 4 elements");
     const Plan pl = make_plan(p);
-    SFAST_REQUIRE(pl.nblk <= (1ll << 30) && pl.nblk * (pl.nsplit > 1 ? 128 : 1) <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
+    // (the join gives a wave to a row: bq rows of a unit)
+    SFAST_REQUIRE(fits_launch(pl.nblk + 7, pl.nw * 128) && (pl.nsplit == 1 || fits_launch(pl.units * 128, 64)), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
     BlockAttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.out_rest = out_rest, a.lse = lse;
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;

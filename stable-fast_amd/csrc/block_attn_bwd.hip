@@ -462,8 +462,8 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
                       "block_attention_backward: gradient strides must be multiples of 4 elements");
     }
     SFAST_REQUIRE(p->dos[1] >= p->D && p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: rows overlap, or their stride is too long");
-    SFAST_REQUIRE((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) <= (1ll << 30) && (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) <= (1ll << 30) &&
-                      padded_rows(p) / p->B <= (1ll << 30) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
+    SFAST_REQUIRE(fits_launch((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) + 7, 256) && fits_launch((int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) + 7, 256) &&
+                      fits_launch(padded_rows(p) / p->B / 16 + 1, 256) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_attention_backward: workspace too small");

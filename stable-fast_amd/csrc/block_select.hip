@@ -262,7 +262,7 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
     __shared__ uint32_t sums[2][WAVES];
     __shared__ int above_s[WAVES], equal_s[WAVES];
     const int lane = threadIdx.x & 63, wave = WAVES == 1 ? 0 : threadIdx.x >> 6;
-    const int row_id = (int)(WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);  // up to 2^30 rows
+    const int row_id = (int)(WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);  // (less than 2^26 rows)
     if (row_id >= n_rows) return;
     const int64_t row = row_id;
     const int count = topk_count(a, row_id / a.nQ / a.Hk);
@@ -411,7 +411,8 @@ static int check_topk(const sfast_block_topk_params *p) {
     SFAST_REQUIRE(p->H % p->Hk == 0, SFAST_ERR_INVALID, "block_topk: %d query heads are no multiple of %d key heads", p->H, p->Hk);
     SFAST_REQUIRE(p->D % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_topk: head dim %d is no multiple of 4", p->D);
     SFAST_REQUIRE(p->nK <= 32768 && p->topk <= 32768, SFAST_ERR_UNSUPPORTED, "block_topk: %d of %d key blocks (up to 32768)", p->topk, p->nK);
-    SFAST_REQUIRE((int64_t)p->B * p->Hk <= 65535 && p->nQ <= (1 << 20) && (int64_t)p->B * p->Hk * p->nQ <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_topk: too many rows");
+    SFAST_REQUIRE((int64_t)p->B * p->Hk <= 65535 && p->nQ <= (1 << 20) &&
+                      fits_launch((int64_t)p->B * p->Hk * p->nQ, p->nK <= 2048 ? 64 : 1024), SFAST_ERR_UNSUPPORTED, "block_topk: too many rows");
     return SFAST_OK;
 }
 
@@ -420,7 +421,7 @@ static int check_topk(const sfast_block_topk_params *p) {
 template <typename T> static int means_launch(MeansArgs &a, int run, hipStream_t st) {
     a.runs = a.H * (a.D / run);
     const int64_t blocks = (int64_t)a.B * a.n * ceil_div(a.runs, 32);
-    SFAST_REQUIRE(blocks <= (1ll << 31) - 1 && (int64_t)a.H * a.D <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_means: too many blocks");
+    SFAST_REQUIRE(fits_launch(blocks, 256) && (int64_t)a.H * a.D <= (1ll << 30), SFAST_ERR_UNSUPPORTED, "block_means: too many blocks");
     const dim3 grid((unsigned)blocks);
     set_kernel_name("block_means[V=%d]", run);
     constexpr int MOST = 16 / sizeof(T);
@@ -442,7 +443,7 @@ extern "C" int sfast_hip_block_means(const void *x, const int32_t *lengths, floa
     SFAST_REQUIRE(p->dtype == SFAST_F16 || p->dtype == SFAST_BF16 || p->dtype == SFAST_F32, SFAST_ERR_UNSUPPORTED, "block_means: bad dtype %d", p->dtype);
     MeansArgs a{};
     a.x = x, a.lengths = lengths, a.out = out;
-    a.B = p->B, a.S = p->S, a.H = p->H, a.D = p->D, a.block = p->block, a.n = ceil_div(p->S, p->block);
+    a.B = p->B, a.S = p->S, a.H = p->H, a.D = p->D, a.block = p->block, a.n = (int)ceil_div64(p->S, p->block);
     // 16-byte loads where head dim, strides and address allow them, else element by element
     const int es = (int)dtype_bytes(p->dtype);
     int run = 16 / es;

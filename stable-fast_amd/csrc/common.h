@@ -156,6 +156,8 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 static inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// a launch has fewer than 2^32 threads along each axis of its grid
+static inline bool fits_launch(int64_t workgroups, int threads) { return workgroups * threads < (1ll << 32); }
 static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 static inline bool aligned16(const void *p) { return (((uintptr_t)p) & 15) == 0; }
 static inline bool aligned8(const void *p) { return (((uintptr_t)p) & 7) == 0; }

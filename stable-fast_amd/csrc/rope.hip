@@ -179,7 +179,7 @@ extern "C" int sfast_hip_rope_nd(const void *q, const void *k, const void *posit
     // tokens of a workgroup: enough to give every thread a table entry, few enough to leave eight workgroups for each compute unit
     a.tok = 1;
     while (a.tok < ROPE_MAX_TOK && a.tokens / (2 * a.tok) >= 2048) a.tok *= 2;
-    SFAST_REQUIRE(ceil_div64(a.tokens, a.tok) <= (1ll << 31) - 1, SFAST_ERR_UNSUPPORTED, "rope_nd: too many tokens");
+    SFAST_REQUIRE(fits_launch(ceil_div64(a.tokens, a.tok), 256), SFAST_ERR_UNSUPPORTED, "rope_nd: too many tokens");
     hipStream_t st = (hipStream_t)stream;
     const int v = p->interleaved ? run / 2 : run;
     set_kernel_name("rope_nd[%s,V=%d]", p->interleaved ? "pairs" : "halves", v);

@@ -127,6 +127,27 @@ def test_block_attention_refuses_rows_that_overlap(built_lib, name):
     assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, 1 << 40, None) == -1
 
 
+def test_calls_beyond_a_launch_are_refused(built_lib):
+    """A grid has fewer than 2^32 threads along an axis."""
+    from sfast.hip import lib as L
+    lib = L.load()
+    s = (C.c_int64 * 3)(1 << 40, 64, 64)
+    p = L.RopeParams(L.BF16, 2, 1 << 29, 1, 1, 64, 1, (C.c_int32 * 4)(64), 1, 0, L.POS_I64, 10000.0, s, s, s, s, (C.c_int64 * 2)(0, 1))
+    assert lib.sfast_hip_rope_nd(4096, 4096, 4096, 4096, 4096, C.byref(p), None) == -1
+    p = L.BlockMeansParams(L.BF16, 1, (1 << 31) - 1, 1, 64, 64, s)
+    assert lib.sfast_hip_block_means(4096, None, 4096, C.byref(p), None) == -1
+    p = L.BlockTopkParams(8, 1 << 20, 4096, 1, 1, 64, 8, 64)
+    assert lib.sfast_hip_block_topk(4096, 4096, None, 4096, C.byref(p), 4096, 1 << 60, None) == -1
+    p = attn_params(L, Sq=1 << 30, H=4, Hk=4, B=2, topk=1)
+    args = [4096, 4096, 4096, 4096, None, None, 4096, 4096, None]
+    assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, 1 << 60, None) == -1
+    p = attn_params(L, Sq=1 << 27, H=4, topk=2000)      # lists that are cut: a second launch has a wave for every row
+    assert lib.sfast_hip_block_attention(*args, C.byref(p), 4096, 1 << 60, None) == -1
+    back = [4096, 4096, 4096, 4096, None, None, 4096, None, 4096, 4096, None, 4096, 4096, 4096]
+    p = attn_params(L, Sq=1 << 28, topk=1)
+    assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, 1 << 60, None) == -1
+
+
 def test_the_choice_refuses_lists_longer_than_any_row(built_lib):
     """(the entries behind the last block are filled with -1 in steps of 32-bit indexes)"""
     from sfast.hip import lib as L
