@@ -22,7 +22,8 @@ template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + 2 
 
 // What a row's statistics enter the dkv kernel's products as: -lse / scale and -delta, each as four numbers of the type times fixed powers of
 // two (one more matrix instruction starts the accumulators from their sums). Together they hold 32 bits and more; parts below the type's
-// normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied.
+// normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied. A finite number beyond them (f16: 2^31,
+// where q . k holds no more than its leading digits unless scale is tiny) becomes NaN: a gradient that cannot be had is not 0.
 constexpr float BB_PART[4] = {32768.f, 16.f, 1.f / 128.f, 1.f / 16384.f};
 template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
     typename Elem<T>::vec4 v;
@@ -31,6 +32,7 @@ template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
         float a = x * (1.f / BB_PART[i]);
         if (fabsf(a) < 6.103515625e-5f) a = 0.f;
         v[i] = Elem<T>::from_f32(a);
+        if (i == 0 && fabsf(x) < INFINITY && fabsf((float)v[0]) == INFINITY) v[0] = Elem<T>::from_f32(NAN);
         const float taken = (float)v[i];
         x = taken != taken || fabsf(taken) == INFINITY ? 0.f : fmaf(-taken, BB_PART[i], x);
     }

@@ -793,7 +793,10 @@ def block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, ls
                                     scale: Optional[float] = None, out_rest=None):
     """Gradients (dq, dk, dv) of block_sparse_attention from its results, the gradient of out and that of lse (or None). out_rest: what the
     rounding of out left behind (autograd keeps it), without which rows that attend to few keys lose some accuracy. The same call gives the
-    same bits."""
+    same bits. f16: |lse / scale| and |delta| below 2^31 (NaN beyond), products of grad_out and v within the type.
+
+    To capture a training step, capture this call, or the backward of results that were made inside the capture: torch cannot capture
+    the backward of an eager graph, nor one beside which an eager graph of the same leaves is alive."""
     L.load_torch_ops()
     return torch.ops.sfast_xformers.block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q, block_k, key_lengths,
                                                                     query_lengths, scale, out_rest)

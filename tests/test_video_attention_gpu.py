@@ -338,6 +338,23 @@ def test_block_attention_strides(dtype, grads):
     attend(case, heads_first, kv[:, :, 0], kv[:, :, 1], wide, grads=grads)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_block_attention_gradients_of_far_scores_under_a_tiny_scale(dtype):
+    """q . k of -3 * 10^9 (D elements of magnitude 5000 each way) with a scale that makes it -3: f16 has no way to hold -lse / scale, which
+    is said with a NaN, not with a zero; bf16 does it."""
+    D = 128
+    q = torch.full((1, 1, 1, D), 5000.0, dtype=dtype, device="cuda")
+    k = torch.full((1, 2, 1, D), -5000.0, dtype=dtype, device="cuda")
+    v = torch.ones(1, 2, 1, D, dtype=dtype, device="cuda")
+    blocks = torch.zeros(1, 1, 1, 1, dtype=torch.int32, device="cuda")
+    out, lse = F.block_sparse_attention(q, k, v, blocks, scale=1e-9)
+    dq, dk, dv = F.block_sparse_attention_backward(torch.ones_like(out), None, q, k, v, blocks, out, lse, scale=1e-9)
+    if dtype == F16:
+        assert torch.isnan(dv).all()
+    else:
+        assert torch.equal(dv, torch.full_like(dv, 0.5))
+
+
 def test_block_attention_rows_that_overlap():
     """Rows that share memory (windows over a line of numbers), the last one with an infinity: it stays in its own column."""
     D, S = 16, 5
