@@ -349,7 +349,7 @@ static Plan make_plan(const sfast_block_attn_params *p) {
         const double part = 2.0 * units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
         const auto tile_us = [&](int64_t blocks) { return pl.pack || blocks <= 256 ? 0.8 : 1.1; };
         double best = tile_us(units * least) * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
-        for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * units <= 1024; ++x) {
+        for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * units <= 1024; x += 1 + x / 32) {
             const double rounds = (double)ceil_div64(x * units, 512);
             const double t = tile_us(x * units) * (double)ceil_div64(tiles, x) * rounds + 4.0 + part * (double)x;
             if (t < best) best = t, ns = x;
