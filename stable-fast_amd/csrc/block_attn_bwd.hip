@@ -18,6 +18,7 @@ constexpr int BB_LIST = 1024, BB_NAMES = 256;  // list entries, query blocks hel
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 16; }
+template <int DP> constexpr int bb_halves() { return DP == 64 ? 2 : 1; }  // waves that share the rows of a dkv tile (64-key blocks)
 template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + 2 * 1024 + BB_NAMES * 2 * 4 + 16; }
 
 // What a row's statistics enter the dkv kernel's products as: -lse / scale and -delta, each as four numbers of the type times fixed powers of
@@ -227,12 +228,12 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
 
 // dK and dV of one key block: NW waves of 32 keys (K and V in registers as the lanes' columns), streaming 64-row tiles of Q and dO of the query
 // blocks that name it, of all heads of the group
-template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dkv_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(NW * RS * 64, DP == 128 ? 1 : RS + 1) block_attn_dkv_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
-    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, NT = NW * 64;
+    constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     char *const stat = smem + 4 * TILE;                           // two stages of 64 rows' parts
-    int *names = reinterpret_cast<int *>(stat + 2 * 1024);        // query block, count of it
+    int *names = reinterpret_cast<int *>(stat + 2 * 1024);        // query block, log2 of how often it names the key block
     int *n_p = names + 2 * BB_NAMES;
 
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
@@ -242,7 +243,8 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
     const int hk = pair % a.Hk, b = pair / a.Hk;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
-    const int64_t key = (int64_t)j * a.bk + wave * 32 + l31;
+    const int kw = RS == 1 ? wave : wave % NW, half = RS == 1 ? 0 : wave / NW;
+    const int64_t key = (int64_t)j * a.bk + kw * 32 + l31;
     const bool key_ok = key < klen;
 
     const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + key * a.ks[1] + (int64_t)hk * a.ks[2];
@@ -259,7 +261,7 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
         kf[kd] = __builtin_bit_cast(vec8, x);
         vf[kd] = __builtin_bit_cast(vec8, y);
     }
-    BaLoader<DP, NW> ql, gl;
+    BaLoader<DP, NW * RS> ql, gl;
     ql.init(wave, lane, a.qs[1], a.D);
     gl.init(wave, lane, a.dos[1], a.D);
     vec8 powers;  // B operand of the statistics' parts
@@ -271,20 +273,37 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
 #pragma unroll
         for (int i = 0; i < 16; ++i) dk[db][i] = 0.f, dv[db][i] = 0.f;
     const float c = a.c;
-    const int subs = a.bq >> 6, per = a.G * subs;
+    const int subs = a.bq >> 6;
     const int32_t *cnt = a.cnt + ((int64_t)pair * a.nK + j) * a.nQ;
 
-    // step x of a list: entry x / per, head (x % per) / subs, 64-row tile x % subs of the query block
-    const auto request = [&](int x, int stage) __attribute__((always_inline)) {
-        const int e = x / per, y = x - e * per, g = y / subs, sub = y - g * subs;
-        const int qb = __builtin_amdgcn_readfirstlane(names[2 * e]);
-        const int h = hk * a.G + g, s0 = qb * a.bq + sub * 64;
+    // the step that is requested next: entry e of the list (query block qb, log2 of its count), head g of the group, 64-row tile sub of the block
+    int e = 0, g = 0, sub = 0, qb = 0, often = 0, entries = 0;
+    const T *Qh = nullptr, *Gh = nullptr;  // the head's rows
+    const u32x4 *Sh = nullptr;
+    const auto entry = [&]() __attribute__((always_inline)) {
+        qb = __builtin_amdgcn_readfirstlane(names[2 * e]), often = __builtin_amdgcn_readfirstlane(names[2 * e + 1]);
+    };
+    const auto first_head = [&]() __attribute__((always_inline)) {
+        const int64_t h = (int64_t)hk * a.G;
+        Qh = (const T *)a.q + (int64_t)b * a.qs[0] + h * a.qs[2];
+        Gh = (const T *)a.dout + (int64_t)b * a.dos[0] + h * a.dos[2];
+        Sh = a.stat + ((int64_t)b * a.H + h) * (a.nQ * a.bq);
+    };
+    const auto request = [&](int stage) __attribute__((always_inline)) {
+        const int s0 = qb * a.bq + sub * 64;
         char *Qs = smem + stage * (2 * TILE);
-        ql.load((const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)h * a.qs[2], a.qs[1], a.D, s0, qlen - s0, Qs, wave);
-        gl.load((const T *)a.dout + (int64_t)b * a.dos[0] + (int64_t)h * a.dos[2], a.dos[1], a.D, s0, qlen - s0, Qs + TILE, wave);
-        if (wave == NW - 1) {
-            const u32x4 *rows = a.stat + ((int64_t)b * a.H + h) * (a.nQ * a.bq) + s0;
-            ba_dma(ba_rsrc(rows, 1024), (ba_lds_t)(stat + stage * 1024), lane * 16);
+        ql.load(Qh, a.qs[1], a.D, s0, qlen - s0, Qs, wave);
+        gl.load(Gh, a.dos[1], a.D, s0, qlen - s0, Qs + TILE, wave);
+        if (wave == NW * RS - 1) ba_dma(ba_rsrc(Sh + s0, 1024), (ba_lds_t)(stat + stage * 1024), lane * 16);
+        if (++sub == subs) {
+            sub = 0;
+            if (++g == a.G) {
+                g = 0, ++e;
+                first_head();
+                if (e < entries) entry();
+            } else {
+                Qh += a.qs[2], Gh += a.dos[2], Sh += a.nQ * a.bq;
+            }
         }
     };
 
@@ -297,67 +316,95 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                 const int m = i + lane < min(i0 + BB_NAMES, i_all) ? cnt[i + lane] : 0;
                 const uint64_t some = __ballot(m > 0);
                 const int at = n + __popcll(some & ((1ull << lane) - 1));
-                if (m > 0) names[2 * at] = i + lane, names[2 * at + 1] = m;
+                if (m > 0) names[2 * at] = i + lane, names[2 * at + 1] = __float_as_int(__log2f((float)m));
                 n += __popcll(some);
             }
             if (lane == 0) *n_p = n;
         }
         __syncthreads();
-        const int steps = __builtin_amdgcn_readfirstlane(*n_p) * per;
-        if (steps > 0) request(0, 0);
+        entries = __builtin_amdgcn_readfirstlane(*n_p);
+        const int steps = entries * (a.G * subs);
+        e = 0, g = 0, sub = 0;
+        first_head();
+        int often_now = 0, often_next = 0;
+        if (steps > 0) {
+            entry();
+            often_next = often;
+            request(0);
+        }
         for (int x = 0; x < steps; ++x) {
             const char *Qs = smem + (x & 1) * (2 * TILE), *Gs = Qs + TILE;
             const char *Ls = stat + (x & 1) * 1024;
-            const int count = __builtin_amdgcn_readfirstlane(names[2 * (x / per) + 1]);
             ba_sync();
-            if (x + 1 < steps) request(x + 1, (x + 1) & 1);
+            often_now = often_next, often_next = often;
+            const float times = __int_as_float(often_now);  // exp2(x + times) = count exp2(x)
+            if (x + 1 < steps) request((x + 1) & 1);
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                vec8 qf[KD], gf[KD], qt[2][DB], gt[2][DB];
+            for (int y = 0; y < 2 / RS; ++y) {
+                const int rb = RS == 1 ? y : half;
+                vec8 qf[KD], gt[2][DB];
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) {
-                    qf[kd] = ba_row_frag<T, DP>(Qs, rb * 32 + l31, kd, hi);
-                    gf[kd] = ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int kd = 0; kd < KD; ++kd) qf[kd] = ba_row_frag<T, DP>(Qs, rb * 32 + l31, kd, hi);
                 const u32x4 parts = *reinterpret_cast<const u32x4 *>(Ls + (rb * 32 + l31) * 16);
                 f32x16 sc, dp;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
-                // s - lse / scale and dP - delta
+                for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+                // s - lse / scale
                 sc = ba_mfma(__builtin_bit_cast(vec8, u32x4{hi ? 0u : parts[0], hi ? 0u : parts[1], 0u, 0u}), powers, sc);
-                dp = ba_mfma(__builtin_bit_cast(vec8, u32x4{hi ? 0u : parts[2], hi ? 0u : parts[3], 0u, 0u}), powers, dp);
 #pragma unroll
-                for (int kd = 0; kd < KD; ++kd) {
-                    sc = ba_mfma(qf[kd], kf[kd], sc);
-                    dp = ba_mfma(gf[kd], vf[kd], dp);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int kd = 0; kd < KD; ++kd) sc = ba_mfma(qf[kd], kf[kd], sc);
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        gt[g][db] = ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16);
-                        qt[g][db] = ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
+                    for (int db = 0; db < DB; ++db) gt[g][db] = ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16);
                 vec8 p8[2], ds[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float p = __builtin_amdgcn_exp2f(sc[i] * c);
-                    if (count != 1) p *= (float)count;
-                    p8[i >> 3][i & 7] = Elem<T>::from_f32(p);
-                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * dp[i]);
+                    sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c, times));
+                    p8[i >> 3][i & 7] = Elem<T>::from_f32(sc[i]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        dv[db] = ba_mfma(gt[g][db], p8[g], dv[db]);
-                        dk[db] = ba_mfma(qt[g][db], ds[g], dk[db]);
-                    }
+                    for (int db = 0; db < DB; ++db) dv[db] = ba_mfma(gt[g][db], p8[g], dv[db]);
+                vec8 gf[KD], qt[2][DB];
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) gf[kd] = ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = 0.f;
+                // dP - delta
+                dp = ba_mfma(__builtin_bit_cast(vec8, u32x4{hi ? 0u : parts[2], hi ? 0u : parts[3], 0u, 0u}), powers, dp);
+#pragma unroll
+                for (int kd = 0; kd < KD; ++kd) dp = ba_mfma(gf[kd], vf[kd], dp);
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) qt[g][db] = ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[i >> 3][i & 7] = Elem<T>::from_f32(sc[i] * dp[i]);
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) dk[db] = ba_mfma(qt[g][db], ds[g], dk[db]);
             }
         }
+    }
+    if constexpr (RS == 2) {
+        // the second half's sums come through LDS (the stages are free)
+        __syncthreads();
+        float *const so = reinterpret_cast<float *>(smem) + kw * (2 * DB * 16 * 64) + lane;
+        if (half == 1) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) so[(db * 16 + i) * 64] = dk[db][i], so[((DB + db) * 16 + i) * 64] = dv[db][i];
+        }
+        __syncthreads();
+        if (half == 1) return;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) dk[db][i] += so[(db * 16 + i) * 64], dv[db][i] += so[((DB + db) * 16 + i) * 64];
     }
     if (key >= a.Sk) return;
     T *Kg = (T *)a.dk + (int64_t)b * a.dks[0] + key * a.dks[1] + (int64_t)hk * a.dks[2];
@@ -385,8 +432,8 @@ template <typename T, int DP> int set_attr() {
     };
     one((const void *)block_attn_dq_kernel<T, DP, 2>, bb_dq_lds<DP>());
     one((const void *)block_attn_dq_kernel<T, DP, 4>, bb_dq_lds<DP>());
-    one((const void *)block_attn_dkv_kernel<T, DP, 2>, bb_dkv_lds<DP>());
-    one((const void *)block_attn_dkv_kernel<T, DP, 4>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>()>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 4, 1>, bb_dkv_lds<DP>());
     if (e != hipSuccess) {
         set_error("hipFuncSetAttribute(block_attn_bwd): %s", hipGetErrorString(e));
         return SFAST_ERR_LAUNCH;
@@ -417,9 +464,9 @@ template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
     a.nblk = a.B * a.Hk * a.nK;
     a.chunk = ceil_div(a.nblk, 8);
     if (a.bk == 64)
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2>), dim3(8 * a.chunk), dim3(128), bb_dkv_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>()>), dim3(8 * a.chunk), dim3(128 * bb_halves<DP>()), bb_dkv_lds<DP>(), st, a);
     else
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4, 1>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
     return check_launch("block_attention_backward dkv");
 }
 
