@@ -20,11 +20,13 @@ constexpr int BA_MAX_LIST = 1024;  // entries of one workgroup's (part of a) lis
 template <int DP, int NS> constexpr int ba_fwd_lds() { return NS * 2 * BaTile<DP>::BYTES + BA_MAX_LIST * 2 * 4 + 16; }
 
 // NS: LDS stages, NS - 1 tiles are on their way while one is used. KW = 2: two waves share the rows and take a half of every tile's keys each
-// (joined through LDS at the end): where compute units are not full, a tile's chain of products, softmax and products is what takes time.
+// (joined through LDS at the end): where compute units are not full, a tile's chain of products, softmax and products is what takes time, and
+// with 64 rows a workgroup its LDS leaves room for half the waves otherwise (16384 x 16 rows of 128, blocks of 64: 410 -> 340 us; with 128
+// rows the waves are there anyway and the second set of them costs more than it hides, 177 -> 195 us for 14400 x 20 rows of 64).
 // PACK: rows are (query, head of the group) pairs, row = s * G + g, one unit per key head; else one unit per query head.
-constexpr int ba_key_waves(int NS, bool PACK) { return PACK || NS > 2 ? 2 : 1; }
+constexpr int ba_key_waves(int NW, int NS, bool PACK) { return PACK || NS > 2 || NW == 2 ? 2 : 1; }
 
-template <typename T, int DP, int NW, int NS, bool PACK, int KW = ba_key_waves(NS, PACK)>
+template <typename T, int DP, int NW, int NS, bool PACK, int KW = ba_key_waves(NW, NS, PACK)>
 __global__ void __launch_bounds__(NW * KW * 64, 2) block_attn_fwd_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES, KBN = 2 / KW;
@@ -365,7 +367,7 @@ template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl,
     const dim3 grid((unsigned)(8 * a.chunk));
     const auto go = [&](auto NW, auto NS, auto PACK) {
         constexpr int nw = decltype(NW)::value, ns = decltype(NS)::value;
-        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * ba_key_waves(ns, decltype(PACK)::value) * 64),
+        hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * ba_key_waves(nw, ns, decltype(PACK)::value) * 64),
                            (ba_fwd_lds<DP, ns>()), st, a);
     };
     const auto with = [&](auto NW, auto PACK) {
