@@ -17,10 +17,9 @@ struct BlockAttnArgs {
     void *out, *out_rest, *dq, *dk, *dv;  // out_rest: what the rounding of out left, or NULL
     float *lse;                // [B, H, Sq], natural log
     const float *dlse;         // gradient of lse, or NULL
-    float *delta;              // [B, H, Sq]: rowsum(dout * o) - dlse
     const int32_t *blocks;     // [B, Hk, nQ, topk]
     const int32_t *klen, *qlen;  // [B] or NULL
-    u32x4 *stat;               // backward: [B, H, nQ * bq] a row's lse and delta as parts (block_attn_bwd.hip)
+    u32x4 *stat;               // backward: [B, H, nQ * bq] a row's lse and delta = rowsum(dout * o) - dlse as parts (block_attn_bwd.hip)
     int32_t *cnt;              // backward: [B, Hk, nK, nQ] how often query block i names key block j
     float *part_o, *part_ml;   // split form: unnormalised partial results, (reference, sum) pairs
     int B, H, Hk, G, Sq, Sk, D, nQ, nK, topk, bq, bk, nsplit;

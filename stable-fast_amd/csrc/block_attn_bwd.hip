@@ -21,7 +21,7 @@ template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_
 template <int DP> constexpr int bb_halves() { return DP == 64 ? 2 : 1; }  // waves that share the rows of a dkv tile (64-key blocks)
 template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + 2 * 1024 + BB_NAMES * 2 * 4 + 16; }
 
-// What a row's statistics enter the dkv kernel's products as: -lse / scale and -delta, each as four numbers of the type times fixed powers of
+// What a row's statistics enter the products as: -lse / scale (dkv) and -delta (both), each as four numbers of the type times fixed powers of
 // two (one more matrix instruction starts the accumulators from their sums). Together they hold 32 bits and more; parts below the type's
 // normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied. A finite number beyond them (f16: 2^31,
 // where q . k holds no more than its leading digits unless scale is tiny) becomes NaN: a gradient that cannot be had is not 0.
@@ -38,6 +38,14 @@ template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
         x = taken != taken || fabsf(taken) == INFINITY ? 0.f : fmaf(-taken, BB_PART[i], x);
     }
     return __builtin_bit_cast(u32x2, v);
+}
+
+// the operand that the parts meet: its elements 0 .. 3 of the 16 summed ones are the powers, the rest 0
+template <typename T> __device__ __forceinline__ typename Elem<T>::vec8 bb_powers(int hi) {
+    typename Elem<T>::vec8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_f32(i < 4 && hi == 0 ? BB_PART[i & 3] : 0.f);
+    return v;
 }
 
 // A row's delta (LPR lanes, 8 elements each) and parts; rows up to whole query blocks exist and are marked empty. Clears the counts as well.
@@ -78,7 +86,6 @@ template <typename T, int LPR> __global__ void __launch_bounds__(256) block_attn
         x = L == -INFINITY ? -INFINITY : -L / a.scale;  // a row without keys: probabilities 0
     } else {
         if (a.dlse && s < qlen) sum -= a.dlse[at];
-        if (s < a.Sq) a.delta[at] = sum;
         x = -sum;
     }
     reinterpret_cast<u32x2 *>(a.stat + ((int64_t)b * a.H + h) * Sp + s)[d == 0 ? 0 : 1] = bb_parts<T>(x);
@@ -127,13 +134,15 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
         qf[kd] = __builtin_bit_cast(vec8, x);
         gf[kd] = __builtin_bit_cast(vec8, y);
     }
-    float L = INFINITY, delta = 0.f;  // a row without keys: probabilities 0
+    float L = INFINITY;  // a row without keys: probabilities 0
+    u32x4 dparts = {0u, 0u, 0u, 0u};
     if (row_ok) {
-        const int64_t at = ((int64_t)b * a.H + h) * a.Sq + s;
-        const float v = a.lse[at];
+        const float v = a.lse[((int64_t)b * a.H + h) * a.Sq + s];
         if (v != -INFINITY) L = v * LOG2E;
-        delta = a.delta[at];
+        const u32x4 parts = a.stat[((int64_t)b * a.H + h) * (a.nQ * a.bq) + s];
+        if (hi == 0) dparts = u32x4{parts[2], parts[3], 0u, 0u};
     }
+    const vec8 powers = bb_powers<T>(hi);
     const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
     BaLoader<DP, NW> kl, vl;
@@ -184,6 +193,7 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                 f32x16 sc, dp;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = 0.f, dp[i] = 0.f;
+                dp = ba_mfma(powers, __builtin_bit_cast(vec8, dparts), dp);  // dP - delta
 #pragma unroll
                 for (int kd = 0; kd < KD; ++kd) {
                     sc = ba_mfma(kf[kd], qf[kd], sc);
@@ -204,7 +214,7 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L));
-                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * (dp[i] - delta));
+                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * dp[i]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
@@ -264,9 +274,7 @@ template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(
     BaLoader<DP, NW * RS> ql, gl;
     ql.init(wave, lane, a.qs[1], a.D);
     gl.init(wave, lane, a.dos[1], a.D);
-    vec8 powers;  // B operand of the statistics' parts
-#pragma unroll
-    for (int i = 0; i < 8; ++i) powers[i] = Elem<T>::from_f32(i < 4 && hi == 0 ? BB_PART[i & 3] : 0.f);
+    const vec8 powers = bb_powers<T>(hi);
     f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -471,7 +479,6 @@ template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
 }
 
 static int64_t padded_rows(const sfast_block_attn_params *p) { return (int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) * p->block_q; }
-static int64_t delta_floats(const sfast_block_attn_params *p) { return ((int64_t)p->B * p->H * p->Sq + 3) / 4 * 4; }
 static int64_t cells(const sfast_block_attn_params *p) {
     return (int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) * ceil_div(p->Sq, p->block_q);
 }
@@ -492,7 +499,7 @@ using namespace sfast;
 
 extern "C" size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p) {
     if (block_attn_check(p) != SFAST_OK) return 0;
-    return (size_t)padded_rows(p) * 16 + (size_t)(delta_floats(p) + cells(p)) * 4;
+    return (size_t)padded_rows(p) * 16 + (size_t)cells(p) * 4;
 }
 
 extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
@@ -520,8 +527,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     a.q = q, a.k = k, a.v = v, a.o = out, a.o_rest = out_rest, a.dout = dout, a.lse = const_cast<float *>(lse), a.dlse = dlse, a.dq = dq, a.dk = dk, a.dv = dv;
     a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths;
     a.stat = (u32x4 *)workspace;
-    a.delta = (float *)(a.stat + padded_rows(p));
-    a.cnt = (int32_t *)(a.delta + delta_floats(p));
+    a.cnt = (int32_t *)(a.stat + padded_rows(p));
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
     a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
     for (int i = 0; i < 3; ++i) {
