@@ -101,8 +101,23 @@ __global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnAr
     if (j >= 0 && (int64_t)j * a.bk < klen) atomicAdd(a.cnt + ((int64_t)pair * a.nK + j) * a.nQ + qb, 1);
 }
 
+// Probabilities and dS are rounded to the type for the products that sum them, which about doubles the square of a gradient's error (1.42 times
+// one rounding's). With FINE the part that this rounding cuts off takes part as well, in products of its own: the gradient keeps its last
+// rounding alone. For calls of one query block, whose time is that of a chain of small steps and not of the products.
+template <typename T, bool FINE> struct BbRounded {
+    typename Elem<T>::vec8 v, rest;
+    __device__ __forceinline__ void set(int i, float x) {
+        v[i] = Elem<T>::from_f32(x);
+        if (FINE) rest[i] = Elem<T>::from_f32(x - (float)v[i]);
+    }
+    __device__ __forceinline__ f32x16 times(typename Elem<T>::vec8 a, f32x16 c) const {
+        if (FINE) c = ba_mfma(a, rest, c);
+        return ba_mfma(a, v, c);
+    }
+};
+
 // dQ of one query block: the forward's streams, K read as rows (scores) and transposed (dQ), V as rows (dP)
-template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -210,16 +225,13 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
                     for (int i = 0; i < 16; ++i)
                         if (kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hi >= left) sc[i] = -INFINITY;
                 }
-                vec8 ds[2];
+                BbRounded<T, FINE> ds[2];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L));
-                    ds[i >> 3][i & 7] = Elem<T>::from_f32(p * dp[i]);
-                }
+                for (int i = 0; i < 16; ++i) ds[i >> 3].set(i & 7, __builtin_amdgcn_exp2f(fmaf(sc[i], c, -L)) * dp[i]);
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) dq[db] = ba_mfma(kt[g][db], ds[g], dq[db]);
+                    for (int db = 0; db < DB; ++db) dq[db] = ds[g].times(kt[g][db], dq[db]);
             }
         }
     }
@@ -238,7 +250,7 @@ template <typename T, int DP, int NW> __global__ void __launch_bounds__(NW * 64,
 
 // dK and dV of one key block: NW waves of 32 keys (K and V in registers as the lanes' columns), streaming 64-row tiles of Q and dO of the query
 // blocks that name it, of all heads of the group
-template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(NW * RS * 64, DP == 128 ? 1 : RS + 1) block_attn_dkv_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launch_bounds__(NW * RS * 64, DP == 128 ? 1 : FINE ? 2 : RS + 1) block_attn_dkv_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -365,16 +377,16 @@ template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
                     for (int db = 0; db < DB; ++db) gt[g][db] = ba_col_frag<T, DP>(Gs, lane, db, rb * 32 + g * 16);
-                vec8 p8[2], ds[2];
+                BbRounded<T, FINE> p8[2], ds[2];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c, times));
-                    p8[i >> 3][i & 7] = Elem<T>::from_f32(sc[i]);
+                    p8[i >> 3].set(i & 7, sc[i]);
                 }
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) dv[db] = ba_mfma(gt[g][db], p8[g], dv[db]);
+                    for (int db = 0; db < DB; ++db) dv[db] = p8[g].times(gt[g][db], dv[db]);
                 vec8 gf[KD], qt[2][DB];
 #pragma unroll
                 for (int kd = 0; kd < KD; ++kd) gf[kd] = ba_row_frag<T, DP>(Gs, rb * 32 + l31, kd, hi);
@@ -389,11 +401,11 @@ template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(
 #pragma unroll
                     for (int db = 0; db < DB; ++db) qt[g][db] = ba_col_frag<T, DP>(Qs, lane, db, rb * 32 + g * 16);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i >> 3][i & 7] = Elem<T>::from_f32(sc[i] * dp[i]);
+                for (int i = 0; i < 16; ++i) ds[i >> 3].set(i & 7, sc[i] * dp[i]);
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) dk[db] = ba_mfma(qt[g][db], ds[g], dk[db]);
+                    for (int db = 0; db < DB; ++db) dk[db] = ds[g].times(qt[g][db], dk[db]);
             }
         }
     }
@@ -433,15 +445,15 @@ template <typename T, int DP, int NW, int RS> __global__ void __launch_bounds__(
         }
 }
 
-template <typename T, int DP> int set_attr() {
+template <typename T, int DP, bool FINE> int set_attr() {
     hipError_t e = hipSuccess;
     const auto one = [&](const void *kern, int bytes) {
         if (e == hipSuccess) e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     };
-    one((const void *)block_attn_dq_kernel<T, DP, 2>, bb_dq_lds<DP>());
-    one((const void *)block_attn_dq_kernel<T, DP, 4>, bb_dq_lds<DP>());
-    one((const void *)block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>()>, bb_dkv_lds<DP>());
-    one((const void *)block_attn_dkv_kernel<T, DP, 4, 1>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dq_kernel<T, DP, 2, FINE>, bb_dq_lds<DP>());
+    one((const void *)block_attn_dq_kernel<T, DP, 4, FINE>, bb_dq_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>(), FINE>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 4, 1, FINE>, bb_dkv_lds<DP>());
     if (e != hipSuccess) {
         set_error("hipFuncSetAttribute(block_attn_bwd): %s", hipGetErrorString(e));
         return SFAST_ERR_LAUNCH;
@@ -449,7 +461,7 @@ template <typename T, int DP> int set_attr() {
     return 0;
 }
 
-template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
+template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, hipStream_t st) {
     const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ;
     const int64_t rows = (int64_t)a.nQ * a.bq * a.H;
     if (DP == 64)
@@ -464,17 +476,17 @@ template <typename T, int DP> int launch(BlockAttnArgs a, hipStream_t st) {
     a.nblk = a.B * a.Hk * a.nQ * a.G;
     a.chunk = ceil_div(a.nblk, 8);
     if (a.bq == 64)
-        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 2>), dim3(8 * a.chunk), dim3(128), bb_dq_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 2, FINE>), dim3(8 * a.chunk), dim3(128), bb_dq_lds<DP>(), st, a);
     else
-        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 4>), dim3(8 * a.chunk), dim3(256), bb_dq_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 4, FINE>), dim3(8 * a.chunk), dim3(256), bb_dq_lds<DP>(), st, a);
     rc = check_launch("block_attention_backward dq");
     if (rc) return rc;
     a.nblk = a.B * a.Hk * a.nK;
     a.chunk = ceil_div(a.nblk, 8);
     if (a.bk == 64)
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>()>), dim3(8 * a.chunk), dim3(128 * bb_halves<DP>()), bb_dkv_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>(), FINE>), dim3(8 * a.chunk), dim3(128 * bb_halves<DP>()), bb_dkv_lds<DP>(), st, a);
     else
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4, 1>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4, 1, FINE>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
     return check_launch("block_attention_backward dkv");
 }
 
@@ -486,10 +498,15 @@ static int64_t cells(const sfast_block_attn_params *p) {
 }  // namespace
 
 int block_attn_bwd_init() {
-    int rc = set_attr<f16, 64>();
-    if (!rc) rc = set_attr<f16, 128>();
-    if (!rc) rc = set_attr<bf16, 64>();
-    if (!rc) rc = set_attr<bf16, 128>();
+    int rc = 0;
+#define SFAST_BB_ATTR(T, DP)                           \
+    if (!rc) rc = set_attr<T, DP, false>();            \
+    if (!rc) rc = set_attr<T, DP, true>();
+    SFAST_BB_ATTR(f16, 64)
+    SFAST_BB_ATTR(f16, 128)
+    SFAST_BB_ATTR(bf16, 64)
+    SFAST_BB_ATTR(bf16, 128)
+#undef SFAST_BB_ATTR
     return rc;
 }
 
@@ -537,7 +554,12 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     a.scale = p->scale;
     a.c = p->scale * LOG2E;
     hipStream_t st = (hipStream_t)stream;
-    set_kernel_name("block_attn_bwd[DP=%d]", p->D <= 64 ? 64 : 128);
-    if (p->dtype == SFAST_F16) return p->D <= 64 ? launch<f16, 64>(a, st) : launch<f16, 128>(a, st);
-    return p->D <= 64 ? launch<bf16, 64>(a, st) : launch<bf16, 128>(a, st);
+    const bool fine = a.nQ == 1;
+    set_kernel_name("block_attn_bwd[DP=%d%s]", p->D <= 64 ? 64 : 128, fine ? ",fine" : "");
+#define SFAST_BB(T)                                                                    \
+    if (p->D <= 64) return fine ? launch<T, 64, true>(a, st) : launch<T, 64, false>(a, st); \
+    return fine ? launch<T, 128, true>(a, st) : launch<T, 128, false>(a, st);
+    if (p->dtype == SFAST_F16) { SFAST_BB(f16) }
+    SFAST_BB(bf16)
+#undef SFAST_BB
 }
