@@ -103,7 +103,9 @@ __global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnAr
 
 // Probabilities and dS are rounded to the type for the products that sum them, which about doubles the square of a gradient's error (1.42 times
 // one rounding's). With FINE the part that this rounding cuts off takes part as well, in products of its own: the gradient keeps its last
-// rounding alone. For calls of one query block, whose time is that of a chain of small steps and not of the products.
+// rounding alone. For calls of one query or one key block: there a single probability can weigh most (errors up to 1.9 times one rounding's
+// without it), and the time is that of a chain of small steps (100 x 16 query rows of 64 against 16 blocks of 64: 43.5 -> 47 us; the whole
+// grids would pay a third).
 template <typename T, bool FINE> struct BbRounded {
     typename Elem<T>::vec8 v, rest;
     __device__ __forceinline__ void set(int i, float x) {
@@ -554,7 +556,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     a.scale = p->scale;
     a.c = p->scale * LOG2E;
     hipStream_t st = (hipStream_t)stream;
-    const bool fine = a.nQ == 1;
+    const bool fine = a.nQ == 1 || a.nK == 1;
     set_kernel_name("block_attn_bwd[DP=%d%s]", p->D <= 64 ? 64 : 128, fine ? ",fine" : "");
 #define SFAST_BB(T)                                                                    \
     if (p->D <= 64) return fine ? launch<T, 64, true>(a, st) : launch<T, 64, false>(a, st); \
