@@ -1,14 +1,20 @@
 // Attention over chosen key blocks, gradients (sfast_hip_block_attention_backward).
 //
 // With P = exp(s - lse): dV = P^T dO, dP = dO V^T, dS = P (dP - delta), dQ = scale dS K, dK = scale dS^T Q, delta = rowsum(dO O) - dlse.
-// Bound by the matrix pipe (seven products a tile pair: the scores and dP are made twice) together with the LDS operand reads.
+// Bound by the matrix pipe (seven products a tile pair: the scores and dP are made twice) together with the VALU (an exponential a pair and
+// kernel). bf16: 14400 x 20 rows of 64 against 32 blocks of 64 take 565 us, 935 TFLOP/s over the seven products (dkv takes 3 parts of 5);
+// 32760 x 24 rows of 128 against 64 blocks 6.6 ms, 878 TFLOP/s.
 //
 //   * two kernels instead of atomics, so that the same call gives the same bits: one streams the listed key blocks past a query block (dQ),
 //     one streams the query blocks past a key block (dK, dV).
 //   * the second needs the lists the other way round: a small kernel counts, per key block, how often each query block names it (integer
 //     atomics: their order changes nothing), and the workgroup of a key block walks its row of counts.
 //   * both keep their own rows' operands and sums in registers and read the streamed tiles from LDS as rows (scores, dP) and transposed (sums).
+//   * dkv of 64-key blocks and heads of 64: four waves a workgroup, two for the keys, two for the halves of each tile's rows. The same LDS then
+//     serves twice the waves (three a SIMD): 594 -> 576 us for the 14400 x 20 rows. Heads of 128 fill the registers: one wave a SIMD (dq in
+//     256 registers spills: 6.6 -> 7.2 ms).
 #include "block_attn.h"
+#include <type_traits>
 
 namespace sfast {
 
@@ -49,7 +55,7 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::vec8 bb_power
 }
 
 // A row's delta (LPR lanes, 8 elements each) and parts; rows up to whole query blocks exist and are marked empty. Clears the counts as well.
-// Bound by reading out, what its rounding left, and its gradient once.
+// Bound by reading out, what its rounding left, and its gradient once (14400 x 20 rows of 64: 24 us, 111 MB, 4.6 TB/s).
 template <typename T, int LPR> __global__ void __launch_bounds__(256) block_attn_delta_kernel(const BlockAttnArgs a, int64_t cells) {
     const int64_t blocks = (int64_t)gridDim.x * gridDim.y;
     for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < cells; i += blocks * 256) a.cnt[i] = 0;
@@ -263,12 +269,13 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    const int j = lin % a.nK, pair = lin / a.nK;
+    const int parts_of_block = a.bk / (NW * 32), unit = lin / parts_of_block, k0 = (lin - unit * parts_of_block) * (NW * 32);  // a block's 128 keys may be two workgroups' work
+    const int j = unit % a.nK, pair = unit / a.nK;
     const int hk = pair % a.Hk, b = pair / a.Hk;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
     const int qlen = a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq;
     const int kw = RS == 1 ? wave : wave % NW, half = RS == 1 ? 0 : wave / NW;
-    const int64_t key = (int64_t)j * a.bk + kw * 32 + l31;
+    const int64_t first_key = (int64_t)j * a.bk + k0, key = first_key + kw * 32 + l31;
     const bool key_ok = key < klen;
 
     const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + key * a.ks[1] + (int64_t)hk * a.ks[2];
@@ -329,7 +336,7 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
         }
     };
 
-    const int i_all = (int64_t)j * a.bk < klen ? (qlen + a.bq - 1) / a.bq : 0;
+    const int i_all = first_key < klen ? (qlen + a.bq - 1) / a.bq : 0;
     for (int i0 = 0; i0 < i_all; i0 += BB_NAMES) {
         __syncthreads();
         if (wave == 0) {
@@ -455,6 +462,7 @@ template <typename T, int DP, bool FINE> int set_attr() {
     one((const void *)block_attn_dq_kernel<T, DP, 2, FINE>, bb_dq_lds<DP>());
     one((const void *)block_attn_dq_kernel<T, DP, 4, FINE>, bb_dq_lds<DP>());
     one((const void *)block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>(), FINE>, bb_dkv_lds<DP>());
+    one((const void *)block_attn_dkv_kernel<T, DP, 2, 2, FINE>, bb_dkv_lds<DP>());
     one((const void *)block_attn_dkv_kernel<T, DP, 4, 1, FINE>, bb_dkv_lds<DP>());
     if (e != hipSuccess) {
         set_error("hipFuncSetAttribute(block_attn_bwd): %s", hipGetErrorString(e));
@@ -483,12 +491,22 @@ template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, hipStream_t
         hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 4, FINE>), dim3(8 * a.chunk), dim3(256), bb_dq_lds<DP>(), st, a);
     rc = check_launch("block_attention_backward dq");
     if (rc) return rc;
-    a.nblk = a.B * a.Hk * a.nK;
+    // Where 64 keys a workgroup leave compute units free, the chain of a workgroup's steps is the time: blocks of 128 are two workgroups' work and
+    // every tile's rows are halved (whole backward of 2 x 4 x 9 blocks of 128 keys of 64: 49 -> 42 us; of 8 x 16 blocks of 64 keys of 128: 57 ->
+    // 46; of 8 x 16 blocks of 128 keys of 128: 98 -> 75).
+    const bool few = (int64_t)a.B * a.Hk * a.nK * (a.bk / 64) <= 256;
+    a.nblk = a.B * a.Hk * a.nK * (few ? a.bk / 64 : 1);
     a.chunk = ceil_div(a.nblk, 8);
-    if (a.bk == 64)
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 2, bb_halves<DP>(), FINE>), dim3(8 * a.chunk), dim3(128 * bb_halves<DP>()), bb_dkv_lds<DP>(), st, a);
+    const auto dkv = [&](auto NW, auto RS) {
+        constexpr int nw = decltype(NW)::value, rs = decltype(RS)::value;
+        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, nw, rs, FINE>), dim3(8 * a.chunk), dim3(nw * rs * 64), bb_dkv_lds<DP>(), st, a);
+    };
+    if (few)
+        dkv(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+    else if (a.bk == 64)
+        dkv(std::integral_constant<int, 2>{}, std::integral_constant<int, bb_halves<DP>()>{});
     else
-        hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, 4, 1, FINE>), dim3(8 * a.chunk), dim3(256), bb_dkv_lds<DP>(), st, a);
+        dkv(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
     return check_launch("block_attention_backward dkv");
 }
 

@@ -1,7 +1,7 @@
 // Which key blocks a query block attends to: block means (sfast_hip_block_means) and the choice by their products (sfast_hip_block_topk).
 //
 // Sums and products run in 64 bits: a choice stands on which of two scores is larger, and in 64 bits the order of the additions does not
-// decide that (products of two fp32 means are exact, sums lose 2^-53). The cost is hidden: the means read x once, and the scores are few.
+// decide that (products of two fp32 means are exact, sums lose 2^-53).
 #include "common.h"
 #include <math.h>
 
@@ -12,6 +12,7 @@ namespace {
 // ---- block means ------------------------------------------------------------------------------------------------------------------------
 // Bound by reading x. A workgroup owns one block and 32 runs of V elements (512 bytes of a contiguous token); 8 groups of threads share its
 // rows, each thread keeps several 16-byte loads in flight, and the groups' sums are added in LDS in a fixed order.
+// (57600 x 10 rows of 64 in bf16: 13.4 us, 5.6 TB/s; 4 x 8191 x 8 rows of 128, ragged: 9.7 us, of which 2 are the launch.)
 struct MeansArgs {
     const void *x;
     const int32_t *lengths;
@@ -75,6 +76,9 @@ template <typename T, int V> __global__ void __launch_bounds__(256) block_means_
 // 64-bit MFMAs (16x16x4) on operands read from memory as fp32: a lane reads four consecutive head-dim elements of its row at a time, and the
 // four products of such a group take them in the order the lanes hold them -- any order of the head dim will do as long as both operands
 // share it. A wave owns 16 x MI query blocks and 16 x NJ key blocks; a workgroup's four waves share the query blocks.
+// 450 x 900 blocks of 10 heads of 64 take 22 us: the matrix pipe is busy for 7.3 of them (64 cycles an instruction, all waves in step), the
+// rest is the first loads' way from memory, the keys' way out (32 MB) and the ends of the grid; without the products it still takes 20 us,
+// without the stores 19.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 struct TopkArgs {
@@ -238,6 +242,7 @@ __global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) 
 // the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. It starts below the
 // bits that all keys share and looks at the upper 31 bits first: those settle all but near-ties, for two instructions a key and bit (a
 // comparison's mask would cost wait states on top). Keys equal to the threshold are taken in the order of their index.
+// Bound by those instructions: 4500 rows of 900 take 14 us, about 20 bits of 52 instructions each; 64 rows of 2048 (four waves) 8 us.
 // sum / maximum over a wave, the same in every lane (row shifts by 1, 2, 4, 8, then across the rows of 16: lane 63 holds the result)
 template <int CTRL> __device__ __forceinline__ uint32_t topk_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);

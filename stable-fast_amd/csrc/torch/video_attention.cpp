@@ -1,8 +1,9 @@
 // torch.ops.sfast.rotary_embedding_nd and torch.ops.sfast_xformers.block_* on the C ABI of libsfast_hip.so, with their gradients.
 //
-// Native because these calls are small where they are made once a token: argument checks, allocation and launch cost 5 - 8 us here against
-// 14 - 32 us through ctypes, a gradient 40 us against 200. The rules are those of the Python operators: outputs are fresh tensors, inputs are never written, work
-// goes to the current stream of the input's device, operands a kernel cannot read in place are copied, everything else is refused.
+// Native because these calls are small where they are made once a token: argument checks, allocation and launch cost 6 - 11 us here against
+// 15 - 32 us through ctypes, a call with its gradient 66 - 81 us against 230 - 250 (45 of them are what torch's engine takes for any backward).
+// The rules are those of the Python operators: outputs are fresh tensors, inputs are never written, work goes to the current stream of the
+// input's device, operands a kernel cannot read in place are copied, everything else is refused.
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
