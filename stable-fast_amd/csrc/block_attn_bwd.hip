@@ -14,6 +14,7 @@
 //     serves twice the waves (three a SIMD): 594 -> 576 us for the 14400 x 20 rows. Heads of 128 fill the registers: one wave a SIMD (dq in
 //     256 registers spills: 6.6 -> 7.2 ms).
 #include "block_attn.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace sfast {
@@ -125,7 +126,7 @@ template <typename T, bool FINE> struct BbRounded {
 };
 
 // dQ of one query block: the forward's streams, K read as rows (scores) and transposed (dQ), V as rows (dP)
-template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : NW == 4 ? 3 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -135,7 +136,8 @@ template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    const int g0 = lin % a.G, u = lin / a.G;
+    const int unit = lin / a.nsplit, sp = lin - unit * a.nsplit;
+    const int g0 = unit % a.G, u = unit / a.G;
     const int qb = u % a.nQ, pair = u / a.nQ;
     const int hk = pair % a.Hk, b = pair / a.Hk, h = hk * a.G + g0;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
@@ -178,8 +180,8 @@ template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds
         for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
     const float c = a.c;
 
-    const int e_all = qb * a.bq < qlen ? a.topk : 0;
-    for (int e0 = 0; e0 < e_all; e0 += BB_LIST) {
+    const int e_all = qb * a.bq < qlen ? (int)((int64_t)a.topk * (sp + 1) / a.nsplit) : 0;
+    for (int e0 = (int)((int64_t)a.topk * sp / a.nsplit); e0 < e_all; e0 += BB_LIST) {
         __syncthreads();
         if (wave == 0) {
             const int n = ba_tiles(a.blocks + ((int64_t)pair * a.nQ + qb) * a.topk, e0, min(e0 + BB_LIST, e_all), a.bk, klen, lane, tiles);
@@ -243,6 +245,17 @@ template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds
             }
         }
     }
+    if (a.nsplit > 1) {
+        float *po = a.part_o + ((int64_t)lin * (NW * 32) + wave * 32 + l31) * a.D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = db * 32 + 8 * i + 4 * hi;
+                if (d < a.D) *reinterpret_cast<f32x4 *>(po + d) = f32x4{dq[db][4 * i], dq[db][4 * i + 1], dq[db][4 * i + 2], dq[db][4 * i + 3]};
+            }
+        return;
+    }
     if (s >= a.Sq) return;
     T *Op = (T *)a.dq + (int64_t)b * a.dqs[0] + (int64_t)s * a.dqs[1] + (int64_t)h * a.dqs[2];
     const float k = row_ok ? a.scale : 0.f;
@@ -269,7 +282,8 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
     const int lin = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    const int parts_of_block = a.bk / (NW * 32), unit = lin / parts_of_block, k0 = (lin - unit * parts_of_block) * (NW * 32);  // a block's 128 keys may be two workgroups' work
+    const int piece = lin / a.nsplit, sp = lin - piece * a.nsplit;
+    const int pieces = a.bk / (NW * 32), unit = piece / pieces, k0 = (piece - unit * pieces) * (NW * 32);  // a block's 128 keys may be two workgroups' work
     const int j = unit % a.nK, pair = unit / a.nK;
     const int hk = pair % a.Hk, b = pair / a.Hk;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
@@ -277,6 +291,11 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
     const int kw = RS == 1 ? wave : wave % NW, half = RS == 1 ? 0 : wave / NW;
     const int64_t first_key = (int64_t)j * a.bk + k0, key = first_key + kw * 32 + l31;
     const bool key_ok = key < klen;
+    const int32_t *cnt = a.cnt + ((int64_t)pair * a.nK + j) * a.nQ;
+    const int i_first = (int)((int64_t)a.nQ * sp / a.nsplit);
+    int i_all = first_key < klen ? min((qlen + a.bq - 1) / a.bq, (int)((int64_t)a.nQ * (sp + 1) / a.nsplit)) : 0;
+    // few query blocks leave most of a long cache unnamed: its keys are not read (3 x 13 heads of one token, 21108 keys of 80: 223 -> 127 us)
+    if (i_all - i_first <= 64 && __ballot(i_first + lane < i_all && cnt[i_first + lane] > 0) == 0) i_all = 0;
 
     const T *Kp = (const T *)a.k + (int64_t)b * a.ks[0] + key * a.ks[1] + (int64_t)hk * a.ks[2];
     const T *Vp = (const T *)a.v + (int64_t)b * a.vs[0] + key * a.vs[1] + (int64_t)hk * a.vs[2];
@@ -285,7 +304,7 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
     for (int kd = 0; kd < KD; ++kd) {
         const int d0 = kd * 16 + hi * 8;
         u32x4 x = {0u, 0u, 0u, 0u}, y = {0u, 0u, 0u, 0u};
-        if (key_ok && d0 < a.D) {
+        if (key_ok && i_all > 0 && d0 < a.D) {
             x = *reinterpret_cast<const u32x4 *>(Kp + d0);
             y = *reinterpret_cast<const u32x4 *>(Vp + d0);
         }
@@ -303,7 +322,6 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
         for (int i = 0; i < 16; ++i) dk[db][i] = 0.f, dv[db][i] = 0.f;
     const float c = a.c;
     const int subs = a.bq >> 6;
-    const int32_t *cnt = a.cnt + ((int64_t)pair * a.nK + j) * a.nQ;
 
     // the step that is requested next: entry e of the list (query block qb, log2 of its count), head g of the group, 64-row tile sub of the block
     int e = 0, g = 0, sub = 0, qb = 0, often = 0, entries = 0;
@@ -336,8 +354,7 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
         }
     };
 
-    const int i_all = first_key < klen ? (qlen + a.bq - 1) / a.bq : 0;
-    for (int i0 = 0; i0 < i_all; i0 += BB_NAMES) {
+    for (int i0 = i_first; i0 < i_all; i0 += BB_NAMES) {
         __syncthreads();
         if (wave == 0) {
             int n = 0;
@@ -435,6 +452,20 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
 #pragma unroll
             for (int i = 0; i < 16; ++i) dk[db][i] += so[(db * 16 + i) * 64], dv[db][i] += so[((DB + db) * 16 + i) * 64];
     }
+    if (a.nsplit > 1) {
+        float *po = a.part_o + ((int64_t)lin * (NW * 32) + kw * 32 + l31) * (2 * a.D);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int d = db * 32 + 8 * i + 4 * hi;
+                if (d < a.D) {
+                    *reinterpret_cast<f32x4 *>(po + d) = f32x4{dk[db][4 * i], dk[db][4 * i + 1], dk[db][4 * i + 2], dk[db][4 * i + 3]};
+                    *reinterpret_cast<f32x4 *>(po + a.D + d) = f32x4{dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]};
+                }
+            }
+        return;
+    }
     if (key >= a.Sk) return;
     T *Kg = (T *)a.dk + (int64_t)b * a.dks[0] + key * a.dks[1] + (int64_t)hk * a.dks[2];
     T *Vg = (T *)a.dv + (int64_t)b * a.dvs[0] + key * a.dvs[1] + (int64_t)hk * a.dvs[2];
@@ -454,6 +485,68 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
         }
 }
 
+// the sum of a row's parts, four elements a thread (KV: a key's dk, then its dv)
+template <typename T, bool KV> __global__ void __launch_bounds__(256) block_attn_add_parts_kernel(const BlockAttnArgs a, int rows, int n_rows) {
+    const int runs = (KV ? 2 : 1) * a.D / 4;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int row = (int)(id / runs), run = (int)(id - (int64_t)row * runs);
+    if (row >= n_rows) return;
+    const int unit = row / rows, r = row - unit * rows;  // a query block of a head | a piece of a key block
+    int b, at, h, d = run * 4;
+    bool there;
+    if (KV) {
+        const int pieces = a.bk / rows, block = unit / pieces, pair = block / a.nK;
+        h = pair % a.Hk, b = pair / a.Hk, at = (block - pair * a.nK) * a.bk + (unit - block * pieces) * rows + r;
+        if (at >= a.Sk) return;
+        there = at < (a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk);
+    } else {
+        const int g = unit % a.G, u = unit / a.G, qb = u % a.nQ, pair = u / a.nQ;
+        h = pair % a.Hk * a.G + g, b = pair / a.Hk, at = qb * a.bq + r;
+        if (at >= a.Sq) return;
+        there = at < (a.qlen ? min(max(a.qlen[b], 0), a.Sq) : a.Sq);
+    }
+    const float *p = a.part_o + ((int64_t)unit * a.nsplit * rows + r) * (runs * 4) + d;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < a.nsplit; ++i) sum += *reinterpret_cast<const f32x4 *>(p + (int64_t)i * rows * (runs * 4));
+    const bool value = KV && d >= a.D;
+    if (value) d -= a.D;
+    const float k = value ? 1.f : a.scale;
+    u32x2 x = pack4<T>(sum[0] * k, sum[1] * k, sum[2] * k, sum[3] * k);
+    if (!there) x = u32x2{0u, 0u};  // behind the sequence
+    T *out = (T *)(KV ? value ? a.dv : a.dk : a.dq);
+    const int64_t *st = KV ? value ? a.dvs : a.dks : a.dqs;
+    *reinterpret_cast<u32x2 *>(out + b * st[0] + at * st[1] + h * st[2] + d) = x;
+}
+
+// How the two products of a call are cut: nq, nk parts of a query block's list and of a key block's query blocks (their sums in fp32 meet in
+// the workspace), few: 64 keys a workgroup and halved tiles.
+struct BwdPlan {
+    int nq, nk;
+    bool few;
+    int64_t units_q, units_k, part_floats;
+};
+
+// A workgroup's chain of tiles is the time where there are fewer workgroups than compute units: it is cut so that they fill them, into parts of
+// eight tiles (about 10 us, against 5 for the second launch) and more. (24 heads of 16217 rows of 40 against one block of 120 keys: 372 -> 155 us;
+// 4 x 2 heads of 56 rows of 96 against 47 blocks of 128: 208 -> 63.)
+static BwdPlan bwd_plan(const sfast_block_attn_params *p) {
+    BwdPlan pl{};
+    const int64_t nQ = ceil_div(p->Sq, p->block_q), nK = ceil_div(p->Sk, p->block_k), G = p->H / p->Hk;
+    const int64_t B = g_batch_ref > 0 ? g_batch_ref : p->B;  // (SFAST_BATCH_INVARIANT: a sample's parts are those of the reference batch, common.h)
+    pl.few = B * p->Hk * nK * (p->block_k / 64) <= 256;
+    pl.units_q = (int64_t)p->B * p->H * nQ, pl.units_k = (int64_t)p->B * p->Hk * nK * (pl.few ? p->block_k / 64 : 1);
+    const auto parts = [&](int64_t units, int64_t steps, int64_t most) {
+        const int64_t n = std::min(std::min(256 / std::max<int64_t>(units / p->B * B, 1), steps / 8), most);
+        return (int)std::max<int64_t>(n, 1);
+    };
+    pl.nq = parts(pl.units_q, (int64_t)p->topk * (p->block_k / 64), p->topk);
+    pl.nk = parts(pl.units_k, nQ * std::min<int64_t>(p->topk, nK) / nK * (p->block_q / 64) * G, nQ);
+    const int64_t keys = pl.few ? 64 : p->block_k;
+    pl.part_floats = std::max(pl.nq > 1 ? pl.units_q * pl.nq * p->block_q * p->D : 0, pl.nk > 1 ? pl.units_k * pl.nk * keys * 2 * p->D : 0);
+    return pl;
+}
+
 template <typename T, int DP, bool FINE> int set_attr() {
     hipError_t e = hipSuccess;
     const auto one = [&](const void *kern, int bytes) {
@@ -471,7 +564,7 @@ template <typename T, int DP, bool FINE> int set_attr() {
     return 0;
 }
 
-template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, hipStream_t st) {
+template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, const BwdPlan &pl, hipStream_t st) {
     const int64_t cells = (int64_t)a.B * a.Hk * a.nK * a.nQ;
     const int64_t rows = (int64_t)a.nQ * a.bq * a.H;
     if (DP == 64)
@@ -483,31 +576,40 @@ template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, hipStream_t
     hipLaunchKernelGGL(block_attn_count_kernel, dim3((unsigned)ceil_div(a.nQ * a.topk, 256), a.B * a.Hk), dim3(256), 0, st, a);
     rc = check_launch("block_attention_backward count");
     if (rc) return rc;
-    a.nblk = a.B * a.Hk * a.nQ * a.G;
+    const auto add_parts = [&](auto KV, int64_t units, int rows) {
+        constexpr bool kv = decltype(KV)::value;
+        const int n_rows = (int)(units * rows);
+        hipLaunchKernelGGL((block_attn_add_parts_kernel<T, kv>), dim3((unsigned)ceil_div64((int64_t)n_rows * ((kv ? 2 : 1) * a.D / 4), 256)), dim3(256), 0, st, a, rows, n_rows);
+        return check_launch("block_attention_backward add parts");
+    };
+    a.nsplit = pl.nq;
+    a.nblk = (int)pl.units_q * pl.nq;
     a.chunk = ceil_div(a.nblk, 8);
     if (a.bq == 64)
         hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 2, FINE>), dim3(8 * a.chunk), dim3(128), bb_dq_lds<DP>(), st, a);
     else
         hipLaunchKernelGGL((block_attn_dq_kernel<T, DP, 4, FINE>), dim3(8 * a.chunk), dim3(256), bb_dq_lds<DP>(), st, a);
     rc = check_launch("block_attention_backward dq");
+    if (!rc && pl.nq > 1) rc = add_parts(std::false_type{}, pl.units_q, a.bq);
     if (rc) return rc;
     // Where 64 keys a workgroup leave compute units free, the chain of a workgroup's steps is the time: blocks of 128 are two workgroups' work and
     // every tile's rows are halved (whole backward of 2 x 4 x 9 blocks of 128 keys of 64: 49 -> 42 us; of 8 x 16 blocks of 64 keys of 128: 57 ->
     // 46; of 8 x 16 blocks of 128 keys of 128: 98 -> 75).
-    const bool few = (int64_t)a.B * a.Hk * a.nK * (a.bk / 64) <= 256;
-    a.nblk = a.B * a.Hk * a.nK * (few ? a.bk / 64 : 1);
+    a.nsplit = pl.nk;
+    a.nblk = (int)pl.units_k * pl.nk;
     a.chunk = ceil_div(a.nblk, 8);
     const auto dkv = [&](auto NW, auto RS) {
         constexpr int nw = decltype(NW)::value, rs = decltype(RS)::value;
         hipLaunchKernelGGL((block_attn_dkv_kernel<T, DP, nw, rs, FINE>), dim3(8 * a.chunk), dim3(nw * rs * 64), bb_dkv_lds<DP>(), st, a);
     };
-    if (few)
+    if (pl.few)
         dkv(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
     else if (a.bk == 64)
         dkv(std::integral_constant<int, 2>{}, std::integral_constant<int, bb_halves<DP>()>{});
     else
         dkv(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-    return check_launch("block_attention_backward dkv");
+    rc = check_launch("block_attention_backward dkv");
+    return rc || pl.nk == 1 ? rc : add_parts(std::true_type{}, pl.units_k, pl.few ? 64 : a.bk);
 }
 
 static int64_t padded_rows(const sfast_block_attn_params *p) { return (int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) * p->block_q; }
@@ -536,7 +638,7 @@ using namespace sfast;
 
 extern "C" size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p) {
     if (block_attn_check(p) != SFAST_OK) return 0;
-    return (size_t)padded_rows(p) * 16 + (size_t)cells(p) * 4;
+    return (size_t)padded_rows(p) * 16 + (size_t)(cells(p) + 3) / 4 * 16 + (size_t)bwd_plan(p).part_floats * 4;
 }
 
 extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
@@ -555,7 +657,8 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
                       "block_attention_backward: gradient strides must be multiples of 4 elements");
     }
     SFAST_REQUIRE(p->dos[1] >= p->D && p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: rows overlap, or their stride is too long");
-    SFAST_REQUIRE(fits_launch((int64_t)p->B * p->H * ceil_div(p->Sq, p->block_q) + 7, 256) && fits_launch((int64_t)p->B * p->Hk * ceil_div(p->Sk, p->block_k) + 7, 256) &&
+    const BwdPlan pl = bwd_plan(p);
+    SFAST_REQUIRE(fits_launch(pl.units_q * pl.nq + 7, 256) && fits_launch(pl.units_k * pl.nk + 7, 256) &&
                       fits_launch(padded_rows(p) / p->B / 16 + 1, 256) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
@@ -565,6 +668,7 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths;
     a.stat = (u32x4 *)workspace;
     a.cnt = (int32_t *)(a.stat + padded_rows(p));
+    a.part_o = (float *)(a.cnt + (cells(p) + 3) / 4 * 4);
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;
     a.bq = p->block_q, a.bk = p->block_k, a.nQ = ceil_div(p->Sq, p->block_q), a.nK = ceil_div(p->Sk, p->block_k);
     for (int i = 0; i < 3; ++i) {
@@ -577,8 +681,8 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     const bool fine = a.nQ == 1 || a.nK == 1;
     set_kernel_name("block_attn_bwd[DP=%d%s]", p->D <= 64 ? 64 : 128, fine ? ",fine" : "");
 #define SFAST_BB(T)                                                                    \
-    if (p->D <= 64) return fine ? launch<T, 64, true>(a, st) : launch<T, 64, false>(a, st); \
-    return fine ? launch<T, 128, true>(a, st) : launch<T, 128, false>(a, st);
+    if (p->D <= 64) return fine ? launch<T, 64, true>(a, pl, st) : launch<T, 64, false>(a, pl, st); \
+    return fine ? launch<T, 128, true>(a, pl, st) : launch<T, 128, false>(a, pl, st);
     if (p->dtype == SFAST_F16) { SFAST_BB(f16) }
     SFAST_BB(bf16)
 #undef SFAST_BB

@@ -373,6 +373,17 @@ def test_gradients_of_one_block_keep_one_rounding(Sq, Sk, H, Hk, D, bq, bk, topk
         assert ((g.cpu().double() - w).norm() / w.norm()).item() <= 1.05 * R.half_step(dtype) / 3 ** 0.5, name
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", [
+    (1, 50, 3000, 4, 2, 64, 64, 64, 40, None, None), (2, 130, 2900, 2, 2, 80, 128, 128, 20, [2900, 900], [130, 70]), (1, 1, 2500, 8, 1, 128, 128, 64, 39, None, None),
+    (1, 4000, 100, 4, 2, 64, 64, 64, 2, None, None), (2, 3000, 130, 2, 1, 40, 128, 128, 2, [130, 60], [3000, 1111]), (1, 2500, 200, 2, 2, 128, 128, 128, 1, None, [2400]),
+    (2, 2100, 1, 3, 3, 96, 64, 64, 1, None, [2100, 0]),
+])
+def test_block_attention_gradients_in_parts(case, dtype):
+    """Few query blocks with long lists, few key blocks that many query blocks name: the chain of tiles is cut, parts are added."""
+    attend(case, *make(case, dtype), grads=True)
+
+
 def test_block_attention_rows_that_overlap():
     """Rows that share memory (windows over a line of numbers), the last one with an infinity: it stays in its own column."""
     D, S = 16, 5
