@@ -339,7 +339,7 @@ struct Plan {
 //  * Packed rows: all query rows of a group fit 64 rows of one or two waves.
 //  * A list is split over workgroups where that is shorter. Measured: a workgroup takes 1.1 us a tile while compute units are free (512
 //    workgroups are two on each), 0.8 us with two waves for the keys; a split adds 4 us for the second launch and the partial results' way
-//    through memory at 0.8 bytes / ps.
+//    through memory at 3.2 bytes / ps (8 heads of 1000 rows of 128 against 64 blocks: 33.5 us, with 0.8 bytes / ps in this sum 45.5).
 //  * deep: four LDS stages instead of two and two waves for the keys, for grids that leave one workgroup to a compute unit anyway
 //    (2 x 6 x 1000 rows against 8 blocks of 64: 11.7 us, with two stages and one wave 14.7).
 static Plan make_plan(const sfast_block_attn_params *p) {
@@ -356,7 +356,7 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     int64_t ns = least;
     if (units < 256) {
         const double rows = pl.pack ? (double)p->Sq * G : pl.nw * 32;
-        const double part = 2.0 * units * rows * p->D * 4 / 0.8e6;  // us a part, written and read
+        const double part = 2.0 * units * rows * p->D * 4 / 3.2e6;  // us a part, written and read
         const auto tile_us = [&](int64_t blocks) { return pl.pack || blocks <= 256 ? 0.8 : 1.1; };
         double best = tile_us(units * least) * (double)ceil_div64(tiles, least) + (least > 1 ? 4.0 + part * least : 0.0);
         for (int64_t x = least + 1; x <= p->topk && x <= tiles / 2 && x * units <= 1024; x += 1 + x / 32) {
