@@ -557,7 +557,8 @@ int sfast_hip_block_means(const void *x, const int32_t *lengths, float *out, con
 
 /* Choice of key blocks: out[b][hk][i][:] = the topk blocks j with the largest sum over the group's heads g of qm[b][i][hk * G + g] . km[b][j][hk]
  * (64 bits), among the blocks that begin inside the sequence (j * block_k < key_lengths[b]). Ascending; ties take the lowest j, a NaN score
- * ranks above all; -1 behind the last one. qm: [B, nQ, H, D], km: [B, nK, Hk, D] fp32, contiguous, 16-byte aligned, D % 4 == 0, nK <= 32768. */
+ * ranks above all; -1 behind the last one. qm: [B, nQ, H, D], km: [B, nK, Hk, D] fp32, contiguous, 16-byte aligned, D % 4 == 0, nK and topk
+ * up to 32768. */
 typedef struct {
     int32_t B, nQ, nK, H, Hk, D, topk, block_k;
 } sfast_block_topk_params;
@@ -569,8 +570,8 @@ int sfast_hip_block_topk(const float *qm, const float *km, const int32_t *key_le
  * names: out = softmax(scale q k^T) v, lse[b][h][s] = log sum exp (natural; fp32). An entry outside [0, ceil(key length / block_k)) names
  * nothing, an entry named twice counts twice. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key,
  * give zeros and lse = -inf. Lengths are clipped to [0, S]; NULL: full. q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] (head h reads key head
- * h / (H / Hk)); strides (b, s, h) in elements, multiples of 8, head-dim stride 1, 16-byte aligned bases; D % 8 == 0, D <= 128. out_rest (or
- * NULL; laid out as out) receives what the rounding of out left behind, itself rounded to the type. */
+ * h / (H / Hk)); strides (b, s, h) in elements, multiples of 8, head-dim stride 1, rows D to 2^23 elements apart, 16-byte aligned bases;
+ * D % 8 == 0, D <= 128. out_rest (or NULL; laid out as out) receives what the rounding of out left behind, itself rounded to the type. */
 typedef struct {
     int32_t dtype; /* f16 / bf16 */
     int32_t B, H, Hk, Sq, Sk, D, block_q, block_k, topk;
@@ -585,12 +586,13 @@ int sfast_hip_block_attention(const void *q, const void *k, const void *v, const
                               void *workspace, size_t workspace_bytes, sfast_stream_t stream);
 /* Gradients of the call above from its out, lse and out_rest (or NULL: rowsum(dout * out) then keeps the error of out's rounding, which shows
  * in rows that attend to few keys), the gradient dout of out and (or NULL) dlse of lse [B, H, Sq] fp32. All of dq, dk, dv is
- * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. */
+ * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. f16: NaN where |lse / scale| or
+ * |delta| reaches 2^31. */
 size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p);
 int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
                                        const int32_t *query_lengths, const void *out, const void *out_rest, const float *lse,
-                                       const void *dout, const float *dlse, void *dq, void *dk, void *dv, const sfast_block_attn_params *p, void *workspace, size_t workspace_bytes,
-                                       sfast_stream_t stream);
+                                       const void *dout, const float *dlse, void *dq, void *dk, void *dv, const sfast_block_attn_params *p,
+                                       void *workspace, size_t workspace_bytes, sfast_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,7 @@ namespace sfast {
 
 namespace {
 
-constexpr int BB_LIST = 1024, BB_NAMES = 256;  // list entries, query blocks held in LDS at a time (four dkv workgroups of D <= 64 fit a compute unit)
+constexpr int BB_LIST = 1024, BB_NAMES = 256;  // list entries, query blocks held in LDS at a time (three dkv workgroups of D <= 64 and more fit a compute unit)
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <int DP> constexpr int bb_dq_lds() { return 4 * BaTile<DP>::BYTES + BB_LIST * 2 * 4 + 16; }
