@@ -6,7 +6,8 @@
 // through registers, four in flight a thread.
 //
 // Bound by memory (bf16, q and k): 57600 tokens x 24 heads of 128 take 265 us, 5.3 TB/s (a copy reaches 4.9); with section widths that allow
-// no run longer than a pair 324 us; 10 heads of 64 leave few rows to a token's table, 91 us, 3.2 TB/s. A token of 4 x (32 + 8) heads is a launch.
+// no run longer than a pair 307 us; 10 heads of 64 leave few rows to a token's table, 64 us, 4.6 TB/s (95 in single pairs). No
+// thread divides 64-bit numbers: a workgroup's tokens belong to one sequence (with a division a token those 64 us are 89). A token of 4 x (32 + 8) heads is a launch.
 // Tried: rows of all tokens flattened with the first loads ahead of the table (the table is then read per row: 335 and 92 us), four tokens in
 // flight with their cosines in registers (257 and 105 us).
 #include "common.h"
@@ -25,8 +26,7 @@ struct RopeArgs {
     int n_axes, pos_type, inverse;
     int half0[5];                // first pair of axis a's section (half0[n_axes] = rotated pairs), tail included as a last section
     int64_t qs[3], ks[3], qos[3], kos[3], ps[2];
-    int64_t tokens;              // B * S
-    int tok;                     // tokens of a workgroup
+    int tok, chunks;             // tokens of a workgroup (of one sequence), workgroups of a sequence
     double turn[ROPE_MAX_PAIRS]; // theta^(-2 i / d) / (2 pi) of every pair: angles in turns
 };
 
@@ -47,8 +47,8 @@ template <typename T, int V> struct alignas(sizeof(T) * V) RopeVec {
 template <typename T, int V, bool INTER> __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
     __shared__ float2 table[ROPE_MAX_TOK * ROPE_MAX_PAIRS];
     const int tid = threadIdx.x;
-    const int64_t t0 = (int64_t)blockIdx.x * a.tok;
-    const int ntok = (int)min((int64_t)a.tok, a.tokens - t0);
+    const int b = (int)(blockIdx.x / (uint32_t)a.chunks), s0 = (int)(blockIdx.x - (uint32_t)b * a.chunks) * a.tok;
+    const int ntok = min(a.tok, a.S - s0);
     for (int i = tid; i < ntok * a.pairs; i += 256) {
         const int t = i / a.pairs, p = i - t * a.pairs;
         float2 cs = make_float2(1.f, 0.f);
@@ -56,8 +56,7 @@ template <typename T, int V, bool INTER> __global__ void __launch_bounds__(256) 
             int axis = 0;
 #pragma unroll
             for (int x = 1; x < SFAST_ROPE_MAX_AXES; ++x) axis += x < a.n_axes && p >= a.half0[x];
-            const int64_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
-            const double x = rope_pos(a.pos, a.pos_type, b * a.ps[0] + s * a.ps[1] + axis) * a.turn[p];
+            const double x = rope_pos(a.pos, a.pos_type, b * a.ps[0] + (s0 + t) * a.ps[1] + axis) * a.turn[p];
             double sn, c;
             sincospi(2.0 * (x - rint(x)), &sn, &c);
             cs = make_float2((float)c, a.inverse ? (float)-sn : (float)sn);
@@ -84,7 +83,7 @@ template <typename T, int V, bool INTER> __global__ void __launch_bounds__(256) 
     }
     const int heads = a.H + a.Hk;
     for (int t = 0; t < ntok; ++t) {
-        const int64_t b = (t0 + t) / a.S, s = (t0 + t) - b * a.S;
+        const int s = s0 + t;
         const T *Q = (const T *)a.q + b * a.qs[0] + s * a.qs[1], *K = (const T *)a.k + b * a.ks[0] + s * a.ks[1];
         T *Qo = (T *)a.qo + b * a.qos[0] + s * a.qos[1], *Ko = (T *)a.ko + b * a.kos[0] + s * a.kos[1];
         float2 cs[V];
@@ -120,7 +119,7 @@ template <typename T, int V, bool INTER> __global__ void __launch_bounds__(256) 
 }
 
 template <typename T, int V> static int launch(const RopeArgs &a, bool inter, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div64(a.tokens, a.tok));
+    const dim3 grid((unsigned)(a.B * a.chunks));
     constexpr int MOST = 16 / sizeof(T);  // elements of one access
     if constexpr (2 * V <= MOST) {
         if (inter) hipLaunchKernelGGL((rope_kernel<T, V, true>), grid, dim3(256), 0, st, a);
@@ -180,11 +179,11 @@ extern "C" int sfast_hip_rope_nd(const void *q, const void *k, const void *posit
     }
     SFAST_REQUIRE(!p->interleaved || run >= 2, SFAST_ERR_UNSUPPORTED, "rope_nd: neighbouring pairs need addresses and strides of whole pairs");
     a.ps[0] = p->ps[0], a.ps[1] = p->ps[1];
-    a.tokens = (int64_t)p->B * p->S;
     // tokens of a workgroup: enough to give every thread a table entry, few enough to leave eight workgroups for each compute unit
     a.tok = 1;
-    while (a.tok < ROPE_MAX_TOK && a.tokens / (2 * a.tok) >= 2048) a.tok *= 2;
-    SFAST_REQUIRE(fits_launch(ceil_div64(a.tokens, a.tok), 256), SFAST_ERR_UNSUPPORTED, "rope_nd: too many tokens");
+    while (a.tok < ROPE_MAX_TOK && a.tok < p->S && (int64_t)p->B * p->S / (2 * a.tok) >= 2048) a.tok *= 2;
+    a.chunks = (int)ceil_div64(p->S, a.tok);
+    SFAST_REQUIRE(fits_launch((int64_t)p->B * a.chunks, 256), SFAST_ERR_UNSUPPORTED, "rope_nd: too many tokens");
     hipStream_t st = (hipStream_t)stream;
     const int v = p->interleaved ? run / 2 : run;
     set_kernel_name("rope_nd[%s,V=%d]", p->interleaved ? "pairs" : "halves", v);
