@@ -341,7 +341,8 @@ struct Plan {
 //    workgroups are two on each), 0.8 us with two waves for the keys; a split adds 4 us for the second launch and the partial results' way
 //    through memory at 3.2 bytes / ps (8 heads of 1000 rows of 128 against 64 blocks: 33.5 us, with 0.8 bytes / ps in this sum 45.5).
 //  * deep: four LDS stages instead of two and two waves for the keys, for grids that leave one workgroup to a compute unit anyway
-//    (2 x 6 x 1000 rows against 8 blocks of 64: 11.7 us, with two stages and one wave 14.7).
+//    (2 x 6 x 1000 rows against 8 blocks of 64: 11.7 us, with two stages and one wave 14.7). Not for
+//    packed rows: 4 x 8 of them with lists cut in eight take 19.9 us with four stages, 19.0 with two.
 static Plan make_plan(const sfast_block_attn_params *p) {
     Plan pl{};
     const int G = p->H / p->Hk;
@@ -367,7 +368,7 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     }
     pl.nsplit = (int)ns;
     pl.nblk = pl.units * ns;
-    pl.deep = pl.nblk <= 256;
+    pl.deep = !pl.pack && pl.nblk <= 256;
     return pl;
 }
 
@@ -378,20 +379,20 @@ template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl,
         hipLaunchKernelGGL((block_attn_fwd_kernel<T, DP, nw, ns, decltype(PACK)::value>), grid, dim3(nw * ba_key_waves(nw, ns, decltype(PACK)::value) * 64),
                            (ba_fwd_lds<DP, ns>()), st, a);
     };
-    const auto with = [&](auto NW, auto PACK) {
+    const auto with = [&](auto NW) {
         if (pl.deep)
-            go(NW, std::integral_constant<int, 4>{}, PACK);
+            go(NW, std::integral_constant<int, 4>{}, std::false_type{});
         else
-            go(NW, std::integral_constant<int, 2>{}, PACK);
+            go(NW, std::integral_constant<int, 2>{}, std::false_type{});
     };
     if (pl.pack && pl.nw == 1)
-        with(std::integral_constant<int, 1>{}, std::true_type{});
+        go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{}, std::true_type{});
     else if (pl.pack)
-        with(std::integral_constant<int, 2>{}, std::true_type{});
+        go(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{}, std::true_type{});
     else if (pl.nw == 2)
-        with(std::integral_constant<int, 2>{}, std::false_type{});
+        with(std::integral_constant<int, 2>{});
     else
-        with(std::integral_constant<int, 4>{}, std::false_type{});
+        with(std::integral_constant<int, 4>{});
     int rc = check_launch("block_attention");
     if (rc || pl.nsplit == 1) return rc;
     const int per = pl.pack ? a.Sq * a.G : a.bq;
@@ -433,8 +434,6 @@ int block_attn_init() {
     if (!rc) rc = set_attr<T, DP, 2, 2, true>();                                     \
     if (!rc) rc = set_attr<T, DP, 2, 2, false>();                                    \
     if (!rc) rc = set_attr<T, DP, 4, 2, false>();                                    \
-    if (!rc) rc = set_attr<T, DP, 1, 4, true>();                                     \
-    if (!rc) rc = set_attr<T, DP, 2, 4, true>();                                     \
     if (!rc) rc = set_attr<T, DP, 2, 4, false>();                                    \
     if (!rc) rc = set_attr<T, DP, 4, 4, false>();
     SFAST_BA_ATTR(f16, 64)

@@ -7,7 +7,8 @@
 //
 // Bound by memory (bf16, q and k): 57600 tokens x 24 heads of 128 take 265 us, 5.3 TB/s (a copy reaches 4.9); with section widths that allow
 // no run longer than a pair 307 us; 10 heads of 64 leave few rows to a token's table, 64 us, 4.6 TB/s (95 in single pairs). No
-// thread divides 64-bit numbers: a workgroup's tokens belong to one sequence (with a division a token those 64 us are 89). A token of 4 x (32 + 8) heads is a launch.
+// thread divides 64-bit numbers: a workgroup's tokens belong to one sequence (with a division a token those 64 us are 89). 4 tokens of 24 + 8
+// heads are a launch.
 // Tried: rows of all tokens flattened with the first loads ahead of the table (the table is then read per row: 335 and 92 us); four tokens in
 // flight (247 us, but 75 for the heads of 64 and 330 in single pairs: its registers cost waves).
 #include "common.h"
