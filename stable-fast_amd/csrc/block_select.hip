@@ -240,9 +240,9 @@ __global__ void __launch_bounds__(256) block_score_few_kernel(const TopkArgs a) 
 // ---- the topk best of a row ---------------------------------------------------------------------------------------------------------------
 // WAVES waves hold a row's scores in registers as order-preserving 64-bit keys (0 = not there) and find the topk-th largest bit by bit from
 // the top: a bit stays set while at least topk keys reach the candidate, and the search ends as soon as exactly topk do. It starts below the
-// bits that all keys share and looks at the upper 31 bits first: those settle all but near-ties, for two instructions a key and bit (a
+// bits that all keys in question share and looks at the upper 31 bits first: those settle all but near-ties, for two instructions a key and bit (a
 // comparison's mask would cost wait states on top). Keys equal to the threshold are taken in the order of their index.
-// Bound by those instructions: 4500 rows of 900 take 14 us, about 20 bits of 52 instructions each; 64 rows of 2048 (four waves) 8 us.
+// 4500 rows of 900 take 12 us: about 12 bits of 52 instructions each, and the keys' way in; 64 rows of 2048 (four waves) 8 us.
 // sum / maximum over a wave, the same in every lane (row shifts by 1, 2, 4, 8, then across the rows of 16: lane 63 holds the result)
 template <int CTRL> __device__ __forceinline__ uint32_t topk_dpp(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
@@ -303,22 +303,31 @@ template <int WAVES, int NPL> __global__ void __launch_bounds__(WAVES == 1 ? 256
         }
         big = over_waves(topk_wave_max(big), true);
         small = ~over_waves(topk_wave_max(small), true);
-        const uint32_t differ = big ^ small;
-        const int top = differ ? 31 - __builtin_clz(differ) : -1;
-        edge_up = big & ~((2u << top) - 1u);
-        if (top < 0) edge_up = big;
-        for (int bit = top; bit >= 0; --bit) {
-            const uint32_t cand = edge_up | (1u << bit);
+        const auto reach_up = [&](uint32_t cand) __attribute__((always_inline)) -> uint32_t {
             // 31-bit numbers: the sign of the difference tells which is less; the signs are collected and counted at the end
             uint32_t less = 0;
 #pragma unroll
             for (int n = 0; n < NPL; ++n) less = __builtin_amdgcn_alignbit(less, up[n] - cand, 31);
-            const uint32_t have = (uint32_t)(64 * NPL * WAVES) - over_waves(topk_wave_sum(__builtin_popcount(less)), false);
+            return (uint32_t)(64 * NPL * WAVES) - over_waves(topk_wave_sum(__builtin_popcount(less)), false);
+        };
+        // the topk-th key is mostly within two powers of two of the largest (19 bits of the upper part are its fraction's): one look there
+        // saves the search through the exponents
+        const uint32_t probe = big - (2u << 19);
+        if (big > (2u << 19) && probe > small) {
+            const uint32_t have = reach_up(probe);
+            exact = have == want;
+            if (have >= want)
+                small = edge_up = probe;
+            else
+                big = probe - 1;
+        }
+        const uint32_t differ = big ^ small;
+        const int top = differ ? 31 - __builtin_clz(differ) : -1;
+        if (!exact) edge_up = top < 0 ? big : big & ~((2u << top) - 1u);
+        for (int bit = top; bit >= 0 && !exact; --bit) {
+            const uint32_t cand = edge_up | (1u << bit), have = reach_up(cand);
             if (have >= want) edge_up = cand;
-            if (have == want) {
-                exact = true;
-                break;
-            }
+            exact = have == want;
         }
     }
     if (exact) {
