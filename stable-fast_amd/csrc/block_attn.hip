@@ -461,11 +461,13 @@ extern "C" int sfast_hip_block_attention(const void *q, const void *k, const voi
     SFAST_REQUIRE(q && k && v && blocks && out && lse, SFAST_ERR_INVALID, "block_attention: null argument");
     int rc = block_attn_check(p);
     if (rc != SFAST_OK) return rc;
-    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out) && aligned8(out_rest), SFAST_ERR_UNSUPPORTED, "block_attention: operands must be 16-byte aligned");
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned8(out) && aligned8(out_rest), SFAST_ERR_UNSUPPORTED,
+                  "block_attention: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) SFAST_REQUIRE(p->os[i] % 4 == 0, SFAST_ERR_UNSUPPORTED, "block_attention: output strides must be multiples of 4 elements");
     const Plan pl = make_plan(p);
     // (the join gives a wave to a row: bq rows of a unit)
-    SFAST_REQUIRE(fits_launch(pl.nblk + 7, pl.nw * 128) && (pl.nsplit == 1 || fits_launch(pl.units * 128, 64)), SFAST_ERR_UNSUPPORTED, "block_attention: too many query blocks");
+    SFAST_REQUIRE(fits_launch(pl.nblk + 7, pl.nw * 128) && (pl.nsplit == 1 || fits_launch(pl.units * 128, 64)), SFAST_ERR_UNSUPPORTED,
+                  "block_attention: too many query blocks");
     BlockAttnArgs a{};
     a.q = q, a.k = k, a.v = v, a.blocks = blocks, a.klen = key_lengths, a.qlen = query_lengths, a.out = out, a.out_rest = out_rest, a.lse = lse;
     a.B = p->B, a.H = p->H, a.Hk = p->Hk, a.G = p->H / p->Hk, a.Sq = p->Sq, a.Sk = p->Sk, a.D = p->D, a.topk = p->topk;

@@ -72,7 +72,8 @@ template <typename T, int LPR> __global__ void __launch_bounds__(256) block_attn
         const u32x4 g = *reinterpret_cast<const u32x4 *>((const T *)a.dout + b * a.dos[0] + s * a.dos[1] + h * a.dos[2] + d);
         const u32x4 o = *reinterpret_cast<const u32x4 *>((const T *)a.o + at);
         u32x4 z = {0u, 0u, 0u, 0u};
-        if (a.o_rest) z = *reinterpret_cast<const u32x4 *>((const T *)a.o_rest + at);  // out to 16 more bits: in a row that attends to few keys dP - delta cancels
+        // out to 16 more bits: in a row that attends to few keys dP - delta cancels
+        if (a.o_rest) z = *reinterpret_cast<const u32x4 *>((const T *)a.o_rest + at);
         float x[8], y[8], w[8];
         unpack8<T>(g, x);
         unpack8<T>(o, y);
@@ -126,7 +127,8 @@ template <typename T, bool FINE> struct BbRounded {
 };
 
 // dQ of one query block: the forward's streams, K read as rows (scores) and transposed (dQ), V as rows (dP)
-template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : NW == 4 ? 3 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, bool FINE>
+__global__ void __launch_bounds__(NW * 64, DP == 128 ? 1 : NW == 4 ? 3 : 2) block_attn_dq_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -271,7 +273,8 @@ template <typename T, int DP, int NW, bool FINE> __global__ void __launch_bounds
 
 // dK and dV of one key block: NW waves of 32 keys (K and V in registers as the lanes' columns), streaming 64-row tiles of Q and dO of the query
 // blocks that name it, of all heads of the group
-template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launch_bounds__(NW * RS * 64, DP == 128 ? 1 : FINE ? 2 : RS + 1) block_attn_dkv_kernel(const BlockAttnArgs a) {
+template <typename T, int DP, int NW, int RS, bool FINE>
+__global__ void __launch_bounds__(NW * RS * 64, DP == 128 ? 1 : FINE ? 2 : RS + 1) block_attn_dkv_kernel(const BlockAttnArgs a) {
     using vec8 = typename Elem<T>::vec8;
     constexpr int KD = DP / 16, DB = DP / 32, TILE = BaTile<DP>::BYTES;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -283,7 +286,8 @@ template <typename T, int DP, int NW, int RS, bool FINE> __global__ void __launc
     if ((int)(blockIdx.x >> 3) >= a.chunk || lin >= a.nblk) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
     const int piece = lin / a.nsplit, sp = lin - piece * a.nsplit;
-    const int pieces = a.bk / (NW * 32), unit = piece / pieces, k0 = (piece - unit * pieces) * (NW * 32);  // a block's 128 keys may be two workgroups' work
+    // a block's 128 keys may be two workgroups' work
+    const int pieces = a.bk / (NW * 32), unit = piece / pieces, k0 = (piece - unit * pieces) * (NW * 32);
     const int j = unit % a.nK, pair = unit / a.nK;
     const int hk = pair % a.Hk, b = pair / a.Hk;
     const int klen = a.klen ? min(max(a.klen[b], 0), a.Sk) : a.Sk;
@@ -579,7 +583,8 @@ template <typename T, int DP, bool FINE> int launch(BlockAttnArgs a, const BwdPl
     const auto add_parts = [&](auto KV, int64_t units, int rows) {
         constexpr bool kv = decltype(KV)::value;
         const int n_rows = (int)(units * rows);
-        hipLaunchKernelGGL((block_attn_add_parts_kernel<T, kv>), dim3((unsigned)ceil_div64((int64_t)n_rows * ((kv ? 2 : 1) * a.D / 4), 256)), dim3(256), 0, st, a, rows, n_rows);
+        const dim3 grid((unsigned)ceil_div64((int64_t)n_rows * ((kv ? 2 : 1) * a.D / 4), 256));
+        hipLaunchKernelGGL((block_attn_add_parts_kernel<T, kv>), grid, dim3(256), 0, st, a, rows, n_rows);
         return check_launch("block_attention_backward add parts");
     };
     a.nsplit = pl.nq;
@@ -648,7 +653,8 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     SFAST_REQUIRE(q && k && v && blocks && out && lse && dout && dq && dk && dv, SFAST_ERR_INVALID, "block_attention_backward: null argument");
     int rc = block_attn_check(p);
     if (rc != SFAST_OK) return rc;
-    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(dout) && aligned8(dq) && aligned8(dk) && aligned8(dv),
+    SFAST_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(dout) && aligned8(dq) &&
+                      aligned8(dk) && aligned8(dv),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: operands must be 16-byte aligned");
     for (int i = 0; i < 3; ++i) {
         SFAST_REQUIRE(p->os[i] % 8 == 0 && p->dos[i] % 8 == 0 && p->os[i] >= 0 && p->dos[i] >= 0, SFAST_ERR_UNSUPPORTED,
@@ -659,7 +665,8 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     SFAST_REQUIRE(p->dos[1] >= p->D && p->dos[1] < (1 << 23), SFAST_ERR_UNSUPPORTED, "block_attention_backward: rows overlap, or their stride is too long");
     const BwdPlan pl = bwd_plan(p);
     SFAST_REQUIRE(fits_launch(pl.units_q * pl.nq + 7, 256) && fits_launch(pl.units_k * pl.nk + 7, 256) &&
-                      fits_launch(padded_rows(p) / p->B / 16 + 1, 256) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 && (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
+                      fits_launch(padded_rows(p) / p->B / 16 + 1, 256) && p->B <= 65535 && (int64_t)p->B * p->Hk <= 65535 &&
+                      (int64_t)ceil_div(p->Sq, p->block_q) * p->topk <= (1ll << 30),
                   SFAST_ERR_UNSUPPORTED, "block_attention_backward: too many rows");
     SFAST_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= sfast_hip_block_attention_backward_workspace_bytes(p), SFAST_ERR_WORKSPACE,
                   "block_attention_backward: workspace too small");
