@@ -367,7 +367,7 @@ typedef struct {
     int32_t dtype;
     int32_t B, H, Sq, Skv, D;
     int64_t qs[3], ks[3], vs[3], os[3];
-    float scale;
+    float scale; /* 2^-100 and more, finite */
     int32_t variant;
 } sfast_attn_params;
 

@@ -415,7 +415,8 @@ int block_attn_check(const sfast_block_attn_params *p) {
     SFAST_REQUIRE(p->D % 8 == 0 && p->D <= 128, SFAST_ERR_UNSUPPORTED, "block_attention: head dim %d (a multiple of 8 up to 128 is supported)", p->D);
     SFAST_REQUIRE((p->block_q == 64 || p->block_q == 128) && (p->block_k == 64 || p->block_k == 128), SFAST_ERR_UNSUPPORTED,
                   "block_attention: blocks of 64 or 128 rows, got %d / %d", p->block_q, p->block_k);
-    SFAST_REQUIRE(p->scale > 0.f && p->scale < INFINITY, SFAST_ERR_UNSUPPORTED, "block_attention: the scale must be positive and finite");
+    // (the gradients hold lse / scale in fp32)
+    SFAST_REQUIRE(p->scale >= 0x1p-100f && p->scale < INFINITY, SFAST_ERR_UNSUPPORTED, "block_attention: the scale must be positive (2^-100 and more) and finite");
     SFAST_REQUIRE(p->Sq <= (1 << 30) && p->Sk <= (1 << 30), SFAST_ERR_UNSUPPORTED, "block_attention: more than 2^30 rows");
     for (int i = 0; i < 3; ++i)
         SFAST_REQUIRE(p->qs[i] >= 0 && p->ks[i] >= 0 && p->vs[i] >= 0 && p->qs[i] % 8 == 0 && p->ks[i] % 8 == 0 && p->vs[i] % 8 == 0, SFAST_ERR_UNSUPPORTED,

@@ -280,7 +280,7 @@ struct Attention {
                     who, ": blocks must be int32 [", p.B, ", ", p.Hk, ", ", (p.Sq + block_q - 1) / block_q, ", topk], got ", lists.scalar_type(), " ", lists.sizes());
         p.topk = i32(who, lists.size(3));
         p.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
-        TORCH_CHECK(p.scale > 0.f && std::isfinite(p.scale), who, ": the scale must be positive and finite, got ", p.scale);
+        TORCH_CHECK(p.scale >= 0x1p-100f && std::isfinite(p.scale), who, ": the scale must be positive (2^-100 and more) and finite, got ", p.scale);
         blocks = lists.contiguous();
         klen = lengths_of(who, "key_lengths", key_lengths, p.B, p.Sk, q);
         qlen = lengths_of(who, "query_lengths", query_lengths, p.B, p.Sq, q);

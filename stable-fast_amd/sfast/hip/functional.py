@@ -783,7 +783,7 @@ def block_sparse_attention(q, k, v, blocks, block_q=128, block_k=64, key_lengths
     q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] f16 / bf16, any strides, D % 8 == 0 up to 128; head h reads key head h // (H // Hk). blocks: int32
     [B, Hk, ceil(Sq / block_q), topk], as block_topk returns it: entries outside the sequence (-1) name nothing, an entry named twice counts
     twice. block_q, block_k: 64 or 128. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key, give
-    zeros and lse = -inf. scale: positive, default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq]). Differentiable once in q, k, v;
+    zeros and lse = -inf. scale: positive (2^-100 and more), default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq]). Differentiable once in q, k, v;
     lse may carry a gradient too."""
     L.load_torch_ops()
     return torch.ops.sfast_xformers.block_sparse_attention(q, k, v, blocks, block_q, block_k, key_lengths, query_lengths, scale)

@@ -148,6 +148,15 @@ def test_calls_beyond_a_launch_are_refused(built_lib):
     assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, 1 << 60, None) == -1
 
 
+def test_block_attention_refuses_a_scale_that_lse_cannot_be_divided_by(built_lib):
+    from sfast.hip import lib as L
+    lib = L.load()
+    p = attn_params(L, scale=2.0 ** -101)
+    assert lib.sfast_hip_block_attention(4096, 4096, 4096, 4096, None, None, 4096, 4096, None, C.byref(p), 4096, 1 << 40, None) == -1
+    back = [4096, 4096, 4096, 4096, None, None, 4096, None, 4096, 4096, None, 4096, 4096, 4096]
+    assert lib.sfast_hip_block_attention_backward(*back, C.byref(p), 4096, 1 << 40, None) == -1
+
+
 def test_the_choice_refuses_lists_longer_than_any_row(built_lib):
     """(the entries behind the last block are filled with -1 in steps of 32-bit indexes)"""
     from sfast.hip import lib as L
