@@ -225,10 +225,9 @@ class UNetPlan:
         return {k: {"count": v[0], "gflop": v[1] / 1e9, "mbytes": v[2] / 1e6} for k, v in agg.items()}
 
 
-# hipGraphExec objects that are no longer wanted. A graph is never destroyed in the same breath as its last replay: the HIP runtime releases
-# the kernel commands of a launch on its asynchronous completion thread (ROCclr NDRangeKernelCommand::releaseResources -> free of the
-# captured kernel arguments), and a graph torn down under it ends in an invalid free() on that thread a few milliseconds later -- the
-# backtrace of the round-4 crash (profiles/r05_crash_backtrace_run2.log). Retired graphs are dropped oldest-first, only when more than
+# hipGraphExec objects that are no longer wanted. A graph is never destroyed in the same breath as its last replay: the HIP runtime may
+# still be finishing that launch on its asynchronous completion thread, and graphs torn down under it have ended in an invalid free() on
+# that thread a few milliseconds later (the backtrace: profiles/r05_crash_backtrace_run2.log). Retired graphs are dropped oldest-first, only when more than
 # 2 * _RETIRED_KEEP have piled up, only from capture_plan_graph's own (non-capturing, non-GC) context and only after a device synchronise.
 _RETIRED = collections.deque()
 _RETIRED_KEEP = 8
