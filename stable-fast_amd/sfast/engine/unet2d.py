@@ -190,8 +190,6 @@ class UNetPlan:
         ev = self._fork_events
         if ev is None:
             ev = self._fork_events = {k: torch.cuda.Event() for k in ("fork", LANE_TEMB, LANE_KV, "join")}
-        if FORK_EVENTS_LOCAL:  # A/B knob: the round-4 behaviour (events die inside the capture)
-            ev = {k: torch.cuda.Event() for k in ev}
         ev["fork"].record(main)
         side.wait_event(ev["fork"])
         with torch.cuda.stream(side):
@@ -348,19 +346,15 @@ def capture_plan_graph(plan, stream, pool=None, tail=None, calibrate=True):
             plan.graph_calibration_ms = cal
             if best is None or t < best[0]:
                 best = (t, forked, g)
-    if not GRAPH_DESTROY_LOSER:
-        for _, g in graphs:
-            if g is not best[2]:
-                retire_graph(g, dev)
+    for _, g in graphs:
+        if g is not best[2]:
+            retire_graph(g, dev)
     return OwnedGraph(best[2], dev), best[1]
 
 
 # SFAST_GRAPH_CALIBRATE=0: keep the forked candidate without timing the two graph shapes against each other (52 extra replays of the step:
 # what made the counter passes over the SVD-XT step -- 930 launches each -- run into their timeouts, tools/gpu_pmc_bench.sh)
 GRAPH_CALIBRATE = os.environ.get("SFAST_GRAPH_CALIBRATE", "1") not in ("0", "false", "off", "")
-# A/B knobs of the round-5 crash hunt (tools/crash_repro.py): 1 = the round-4 behaviour
-FORK_EVENTS_LOCAL = os.environ.get("SFAST_FORK_EVENTS_LOCAL", "0") not in ("0", "false", "off", "")
-GRAPH_DESTROY_LOSER = os.environ.get("SFAST_GRAPH_DESTROY_LOSER", "0") not in ("0", "false", "off", "")
 # sfast_epilogue_ext.flags of every GEMM / conv launch of a plan. SFAST_SPLITK_JOIN=1: split-K problems finish inside the GEMM kernel
 # (ticket counters at the end of the plan's workspace) instead of a reduce launch -- off by default, it measured slower on the SD1.5
 # step (one workgroup per tile re-reads all slabs; DESIGN.md round 3, profiles/r03_splitk_join_*.json.log)

@@ -1,8 +1,8 @@
-/* LD_PRELOAD shim for crash hunting on the GPU box (test infrastructure, not product).
+/* LD_PRELOAD shim that prints the backtrace of a thread that dies (test infrastructure, not product).
  *
  * Installs SIGSEGV / SIGABRT / SIGBUS handlers BEFORE Python starts. Python's faulthandler installs its own handlers later and,
  * after dumping the Python stacks, re-raises into the previously installed handler -- this one -- which prints the C backtrace of
- * the FAULTING thread (module + offset, resolvable with llvm-symbolizer / addr2line against the same binaries) together with the
+ * the FAULTING thread (module + offset) together with the
  * thread id and the fault address, then re-raises with the default action so the exit status stays the signal's.
  *
  * Build: gcc -O1 -g -fPIC -shared -o tools/_crashbt.so tools/crashbt.c

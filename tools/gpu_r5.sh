@@ -2,7 +2,7 @@
 # Round-5 GPU sessions (one gpurun call each): tools/gpu_r5.sh <stage> [budget seconds]
 cd "$(dirname "$0")/.."
 mkdir -p gpurun_out
-STAGE=${1:-crash1}
+STAGE=${1:-perf1}
 BUDGET=${2:-780}
 export TMPDIR=/tmp
 T0=$(date +%s)
@@ -15,67 +15,9 @@ run() { # name, timeout, command...
   timeout $to "$@" > gpurun_out/$name.log 2>&1
   echo "exit=$? $(( $(date +%s) - t0 ))s $(tail -n 1 gpurun_out/$name.log | cut -c1-300)" | tee -a gpurun_out/session.log
 }
-# crash hunt: every process under the backtrace shim; glibc's abort text to stderr; Python stacks of all threads
-HUNT="env LD_PRELOAD=$PWD/tools/_crashbt.so LIBC_FATAL_STDERR_=1 PYTHONFAULTHANDLER=1"
-R4SEL="tiny or sd15_unet_parity or compile_drop_in or lcm or live_weight or rccl or add_strided or controlnet"
-hunt() { # tag, per-process timeout, count, command...  -- stops early when the session budget is nearly spent
-  local tag=$1 to=$2 n=$3; shift 3
-  for i in $(seq 1 $n); do
-    [ $(left) -lt $(( to / 2 )) ] && { echo "$tag: budget spent before run $i" >> gpurun_out/session.log; break; }
-    local t0=$(date +%s)
-    timeout $to "$@" > gpurun_out/${tag}_$i.log 2>&1
-    local rc=$?
-    echo "$tag run $i exit=$rc $(( $(date +%s) - t0 ))s $(grep -a -m1 -E 'crashbt\] signal|SENTINEL' gpurun_out/${tag}_$i.log | cut -c1-120) | $(tail -n 1 gpurun_out/${tag}_$i.log | cut -c1-80)" >> gpurun_out/session.log
-    [ $rc -eq 0 ] && rm -f gpurun_out/${tag}_$i.log
-  done
-}
 rm -f gpurun_out/parity.jsonl gpurun_out/session.log
 rocminfo 2>/dev/null | grep -E "gfx|Compute Unit" | head -2 >> gpurun_out/session.log
 case $STAGE in
-crash1)  # (a) the round-4 arrangement, literally: process group inside pytest, chain test inline, events die inside the capture, loser destroyed
-  export SFAST_TEST_INPROC=1
-  SFAST_FORK_EVENTS_LOCAL=1 SFAST_GRAPH_DESTROY_LOSER=1 hunt r4py 300 4 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL"
-  # (b) the amplified reproducer, round-4 behaviour vs this round's
-  SFAST_FORK_EVENTS_LOCAL=1 SFAST_GRAPH_DESTROY_LOSER=1 hunt amp_old 240 3 $HUNT python tools/crash_repro.py --rccl 1 --iters 12 --budget 150
-  hunt amp_new 240 3 $HUNT python tools/crash_repro.py --rccl 1 --iters 12 --budget 150
-  SFAST_FORK_EVENTS_LOCAL=1 SFAST_GRAPH_DESTROY_LOSER=1 hunt r4py_b 300 4 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL"
-  ;;
-crash2)  # backtraces: the round-4 arrangement until it dies twice (once with Python's faulthandler chained in front, once without, so
-  # that the shim sees the original fault address), then this round's default behaviour for the rest of the budget
-  export SFAST_TEST_INPROC=1
-  HUNT_RAW="env LD_PRELOAD=$PWD/tools/_crashbt.so LIBC_FATAL_STDERR_=1"
-  died=0
-  for i in $(seq 1 10); do
-    [ $died -ge 2 ] && break
-    [ $(left) -lt 400 ] && break
-    if [ $(( i % 2 )) -eq 1 ]; then
-      SFAST_FORK_EVENTS_LOCAL=1 SFAST_GRAPH_DESTROY_LOSER=1 hunt r4raw$i 300 1 $HUNT_RAW $PYT -p no:faulthandler tests/test_unet_gpu.py -k "$R4SEL"
-      [ -f gpurun_out/r4raw${i}_1.log ] && died=$(( died + 1 ))
-    else
-      SFAST_FORK_EVENTS_LOCAL=1 SFAST_GRAPH_DESTROY_LOSER=1 hunt r4fh$i 300 1 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL"
-      [ -f gpurun_out/r4fh${i}_1.log ] && died=$(( died + 1 ))
-    fi
-  done
-  hunt r5new 300 20 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL"
-  ;;
-crash3)  # this round's default behaviour in the round-4 arrangement, two fresh pytest processes at a time (the crash is a host-side race:
-  # a second process competing for the cores is a harder test, and the loop takes half the box time), then the norm micro-benchmark
-  export SFAST_TEST_INPROC=1
-  N=${3:-10}
-  for i in $(seq 1 $N); do
-    [ $(left) -lt 200 ] && { echo "r5v: budget spent before round $i" >> gpurun_out/session.log; break; }
-    t0=$(date +%s)
-    ( MASTER_PORT=29533 timeout 400 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL" > gpurun_out/r5v_a$i.log 2>&1; echo $? > gpurun_out/r5v_a$i.rc ) &
-    ( cd . && SFAST_PACKED_WEIGHTS=0 MASTER_PORT=29534 timeout 400 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL" > gpurun_out/r5v_b$i.log 2>&1; echo $? > gpurun_out/r5v_b$i.rc ) &
-    ( cd . && SFAST_PACKED_WEIGHTS=0 MASTER_PORT=29535 timeout 400 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL" > gpurun_out/r5v_c$i.log 2>&1; echo $? > gpurun_out/r5v_c$i.rc ) &
-    wait
-    for v in a b c; do
-      rc=$(cat gpurun_out/r5v_$v$i.rc); rm -f gpurun_out/r5v_$v$i.rc
-      echo "r5v $v$i exit=$rc $(( $(date +%s) - t0 ))s $(grep -a -m1 -E 'crashbt\] signal' gpurun_out/r5v_$v$i.log | cut -c1-120) | $(tail -n 1 gpurun_out/r5v_$v$i.log | cut -c1-80)" >> gpurun_out/session.log
-      [ "$rc" = "0" ] && rm -f gpurun_out/r5v_$v$i.log
-    done
-  done
-  ;;
 perf1)  # round-5 norm kernels (LayerNorm lane groups, GroupNorm two-pass merge): parity first, then per-op and whole-step A/B; the default
   # bench line with the SDXL child (first run of that path); the self-attention mask and the refusal tests
   run t_norm 900 $PYT tests/test_ops_gpu.py -k "group_norm or layer_norm or gn_ or gnstats or stats or fused_groupnorm"
@@ -90,11 +32,6 @@ perf1)  # round-5 norm kernels (LayerNorm lane groups, GroupNorm two-pass merge)
   done
   for f in ab_new1 ab_old1 ab_new2 ab_old2; do echo "$f $(grep -a -o '"value": [0-9.]*' gpurun_out/$f.log | head -1) $(grep -a -o '"ms_per_step": [0-9.]*' gpurun_out/$f.log | head -1)" >> gpurun_out/session.log; done
   [ $(left) -gt 200 ] && run bench_default 400 python bench.py
-  ;;
-armA)  # which of the two round-4 behaviours is sufficient? ONE arm: the fork / join events die inside the capture again
-  # (SFAST_FORK_EVENTS_LOCAL=1), the losing graph is retired as in this round's product -- sequential fresh processes, round-4 arrangement
-  export SFAST_TEST_INPROC=1
-  SFAST_FORK_EVENTS_LOCAL=1 hunt armA 300 40 $HUNT $PYT tests/test_unet_gpu.py -k "$R4SEL"
   ;;
 final3)  # the default bench line FIRST on a fresh box (two final2 sessions in a row measured 150 it/s where every other session of the round
   # measured 180 - 184: is it the box, or what ran before?), then --kernel-trace-only passes (no counters) for the per-symbol durations
