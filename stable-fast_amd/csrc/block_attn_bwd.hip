@@ -686,7 +686,9 @@ extern "C" int sfast_hip_block_attention_backward(const void *q, const void *k, 
     a.c = p->scale * LOG2E;
     hipStream_t st = (hipStream_t)stream;
     const bool fine = a.nQ == 1 || a.nK == 1;
-    set_kernel_name("block_attn_bwd[DP=%d%s]", p->D <= 64 ? 64 : 128, fine ? ",fine" : "");
+    const int dp = p->D <= 64 ? 64 : 128;
+    set_kernel_name("block_attn_bwd[DP=%d,rows=%d,keys=%d,halves=%d,parts=%d+%d%s]", dp, a.bq, pl.few ? 64 : a.bk,
+                    pl.few ? 2 : a.bk == 64 ? (dp == 64 ? bb_halves<64>() : bb_halves<128>()) : 1, pl.nq, pl.nk, fine ? ",fine" : "");
 #define SFAST_BB(T)                                                                    \
     if (p->D <= 64) return fine ? launch<T, 64, true>(a, pl, st) : launch<T, 64, false>(a, pl, st); \
     return fine ? launch<T, 128, true>(a, pl, st) : launch<T, 128, false>(a, pl, st);
