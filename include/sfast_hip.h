@@ -586,8 +586,8 @@ int sfast_hip_block_attention(const void *q, const void *k, const void *v, const
                               void *workspace, size_t workspace_bytes, sfast_stream_t stream);
 /* Gradients of the call above from its out, lse and out_rest (or NULL: rowsum(dout * out) then keeps the error of out's rounding, which shows
  * in rows that attend to few keys), the gradient dout of out and (or NULL) dlse of lse [B, H, Sq] fp32. All of dq, dk, dv is
- * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. f16: NaN where |lse / scale| or
- * |delta| reaches 2^31. */
+ * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. With delta = rowsum(dout * out) - dlse:
+ * bf16 takes gradients of any magnitude; f16 gives NaN where |lse / scale| or |delta| reaches 2^31 and holds delta in steps of 2^-28. */
 size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p);
 int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
                                        const int32_t *query_lengths, const void *out, const void *out_rest, const float *lse,

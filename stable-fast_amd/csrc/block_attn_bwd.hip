@@ -29,20 +29,29 @@ template <int DP> constexpr int bb_halves() { return DP == 64 ? 2 : 1; }  // wav
 template <int DP> constexpr int bb_dkv_lds() { return 4 * BaTile<DP>::BYTES + 2 * 1024 + BB_NAMES * 2 * 4 + 16; }
 
 // What a row's statistics enter the products as: -lse / scale (dkv) and -delta (both), each as four numbers of the type times fixed powers of
-// two (one more matrix instruction starts the accumulators from their sums). Together they hold 32 bits and more; parts below the type's
-// normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied. A finite number beyond them (f16: 2^31,
-// where q . k holds no more than its leading digits unless scale is tiny) becomes NaN: a gradient that cannot be had is not 0.
-constexpr float BB_PART[4] = {32768.f, 16.f, 1.f / 128.f, 1.f / 16384.f};
+// two (one more matrix instruction starts the accumulators from their sums), each number what the ones before it left.
+//  * bf16 has fp32's range: powers of 1, and the numbers hold all of an fp32 value down to bf16's smallest normal number, 2^-126.
+//  * f16: powers 2^15 to 2^-14, from 2^31 down to steps of 2^-28 (a delta below 2^-28 counts as 0; dout is f16 too, in steps of 2^-24, and so
+//    are the gradients). A finite number beyond them (2^31, where q . k holds no more than its leading digits unless scale is tiny) becomes
+//    NaN: a gradient that cannot be had is not 0.
+// Parts below the type's normal numbers are left to the next one, so that nothing depends on how subnormals are multiplied.
+template <typename T> struct BbParts;
+template <> struct BbParts<f16> {
+    static constexpr float POWER[4] = {32768.f, 16.f, 1.f / 128.f, 1.f / 16384.f}, LEAST = 0x1p-14f;
+};
+template <> struct BbParts<bf16> {
+    static constexpr float POWER[4] = {1.f, 1.f, 1.f, 1.f}, LEAST = 0x1p-126f;
+};
 template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
     typename Elem<T>::vec4 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float a = x * (1.f / BB_PART[i]);
-        if (fabsf(a) < 6.103515625e-5f) a = 0.f;
+        float a = x * (1.f / BbParts<T>::POWER[i]);
+        if (fabsf(a) < BbParts<T>::LEAST) a = 0.f;
         v[i] = Elem<T>::from_f32(a);
         if (i == 0 && fabsf(x) < INFINITY && fabsf((float)v[0]) == INFINITY) v[0] = Elem<T>::from_f32(NAN);
         const float taken = (float)v[i];
-        x = taken != taken || fabsf(taken) == INFINITY ? 0.f : fmaf(-taken, BB_PART[i], x);
+        x = taken != taken || fabsf(taken) == INFINITY ? 0.f : fmaf(-taken, BbParts<T>::POWER[i], x);
     }
     return __builtin_bit_cast(u32x2, v);
 }
@@ -51,7 +60,7 @@ template <typename T> __device__ __forceinline__ u32x2 bb_parts(float x) {
 template <typename T> __device__ __forceinline__ typename Elem<T>::vec8 bb_powers(int hi) {
     typename Elem<T>::vec8 v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_f32(i < 4 && hi == 0 ? BB_PART[i & 3] : 0.f);
+    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_f32(i < 4 && hi == 0 ? BbParts<T>::POWER[i & 3] : 0.f);
     return v;
 }
 

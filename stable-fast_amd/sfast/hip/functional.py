@@ -793,7 +793,9 @@ def block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, ls
                                     scale: Optional[float] = None, out_rest=None):
     """Gradients (dq, dk, dv) of block_sparse_attention from its results, the gradient of out and that of lse (or None). out_rest: what the
     rounding of out left behind (autograd keeps it), without which rows that attend to few keys lose some accuracy. The same call gives the
-    same bits. f16: |lse / scale| and |delta| below 2^31 (NaN beyond), products of grad_out and v within the type.
+    same bits. bf16 takes gradients of any magnitude. f16: |lse / scale| and |delta = rowsum(grad_out * out) - grad_lse| below 2^31 (NaN beyond),
+    delta in steps of 2^-28, and dS = P (grad_out . v - delta) in f16 for the products that sum it: infinite beyond 65504, with fewer digits below
+    2^-14, 0 below 2^-25 -- scale the loss so that it stays between.
 
     To capture a training step, capture this call, or the backward of results that were made inside the capture: torch cannot capture
     the backward of an eager graph, nor one beside which an eager graph of the same leaves is alive."""
