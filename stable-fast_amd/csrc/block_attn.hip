@@ -368,7 +368,7 @@ static Plan make_plan(const sfast_block_attn_params *p) {
     }
     pl.nsplit = (int)ns;
     pl.nblk = pl.units * ns;
-    pl.deep = !pl.pack && pl.nblk <= 256;
+    pl.deep = !pl.pack && units * ns <= 256;  // (decides how many waves share a row's keys: the order of its sums)
     return pl;
 }
 
