@@ -196,9 +196,16 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
     return false;
 }
 
+// There are no derivatives in forward mode; a tangent that was left behind would count as zero.
+void no_tangents(const char *who, std::initializer_list<const Tensor *> ts) {
+    for (const Tensor *t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), who, ": there are no derivatives in forward mode (a tensor carries a tangent)");
+}
+
 std::tuple<Tensor, Tensor> rotary_autograd(const Tensor &q, const optional<Tensor> &key, const Tensor &positions, at::IntArrayRef sections, double theta,
                                            bool interleaved, bool inverse) {
     const Tensor k = key ? *key : Tensor();
+    no_tangents("rotary_embedding_nd", {&q, &k, &positions});
     if (!wants_grad({&q, &k})) {
         at::AutoDispatchBelowADInplaceOrView below;
         return rotary(q, key, positions, sections, theta, interleaved, inverse);
@@ -392,6 +399,7 @@ struct BlockSparse : torch::autograd::Function<BlockSparse> {
 std::tuple<Tensor, Tensor> block_sparse_attention_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &blocks, int64_t block_q,
                                                            int64_t block_k, const optional<Tensor> &key_lengths, const optional<Tensor> &query_lengths,
                                                            optional<double> scale) {
+    no_tangents("block_sparse_attention", {&q, &k, &v});
     if (!wants_grad({&q, &k, &v})) {
         at::AutoDispatchBelowADInplaceOrView below;
         return block_sparse_attention(q, k, v, blocks, block_q, block_k, key_lengths, query_lengths, scale);
@@ -400,8 +408,39 @@ std::tuple<Tensor, Tensor> block_sparse_attention_autograd(const Tensor &q, cons
     return {r[0], r[1]};
 }
 
+// gradients computed by the call itself: whoever differentiates them is told
+struct BlockSparseBackward : torch::autograd::Function<BlockSparseBackward> {
+    static variable_list forward(AutogradContext *, const Variable &grad_out, const optional<Variable> &grad_lse, const Variable &q, const Variable &k,
+                                 const Variable &v, const Variable &blocks, const Variable &out, const Variable &lse, int64_t block_q, int64_t block_k,
+                                 const optional<Variable> &key_lengths, const optional<Variable> &query_lengths, optional<double> scale,
+                                 const optional<Variable> &out_rest) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto [dq, dk, dv] = block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q, block_k, key_lengths, query_lengths, scale, out_rest);
+        return {dq, dk, dv};
+    }
+    static variable_list backward(AutogradContext *, variable_list) {
+        TORCH_CHECK(false, "block_sparse_attention_backward: there is no second derivative");
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor> block_sparse_attention_backward_autograd(const Tensor &grad_out, const optional<Tensor> &grad_lse, const Tensor &q,
+                                                                            const Tensor &k, const Tensor &v, const Tensor &blocks, const Tensor &out,
+                                                                            const Tensor &lse, int64_t block_q, int64_t block_k,
+                                                                            const optional<Tensor> &key_lengths, const optional<Tensor> &query_lengths,
+                                                                            optional<double> scale, const optional<Tensor> &out_rest) {
+    const Tensor gl = grad_lse ? *grad_lse : Tensor(), rest = out_rest ? *out_rest : Tensor();
+    no_tangents("block_sparse_attention_backward", {&grad_out, &gl, &q, &k, &v, &out, &lse, &rest});
+    if (!wants_grad({&grad_out, &gl, &q, &k, &v, &out, &lse, &rest})) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return block_sparse_attention_backward(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q, block_k, key_lengths, query_lengths, scale, out_rest);
+    }
+    auto r = BlockSparseBackward::apply(grad_out, grad_lse, q, k, v, blocks, out, lse, block_q, block_k, key_lengths, query_lengths, scale, out_rest);
+    return {r[0], r[1], r[2]};
+}
+
 // the choice takes no gradient: its means are those of the values
 Tensor block_means_autograd(const Tensor &input, int64_t block, const optional<Tensor> &lengths) {
+    no_tangents("block_means", {&input});
     at::AutoDispatchBelowADInplaceOrView below;
     return block_means(input.detach(), block, lengths);
 }
@@ -433,4 +472,5 @@ TORCH_LIBRARY_IMPL(sfast_xformers, CUDA, m) {
 TORCH_LIBRARY_IMPL(sfast_xformers, AutogradCUDA, m) {
     m.impl("block_means", block_means_autograd);
     m.impl("block_sparse_attention", block_sparse_attention_autograd);
+    m.impl("block_sparse_attention_backward", block_sparse_attention_backward_autograd);
 }

@@ -756,7 +756,7 @@ def rotary_nd(q, k, positions, sections: Sequence[int], theta=10000.0, interleav
 
     q: [B, S, H, D], k: [B, S, Hk, D] or None (any strides; f16 / bf16 / f32; D even, up to 256); positions: [S, A] or [B, S, A] int32 / int64 /
     float32 / float64, 1 to 4 axes. interleaved: pairs are neighbours, else the two halves of their section. inverse turns back, which is also
-    the gradient. Returns new tensors (q, k). Differentiable in q and k."""
+    the gradient. Returns new tensors (q, k). Differentiable in q and k (reverse mode; a tensor with a tangent is refused)."""
     L.load_torch_ops()
     return torch.ops.sfast.rotary_embedding_nd(q, k, positions, sections, theta, interleaved, inverse)
 
@@ -783,8 +783,8 @@ def block_sparse_attention(q, k, v, blocks, block_q=128, block_k=64, key_lengths
     q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] f16 / bf16, any strides, D % 8 == 0 up to 128; head h reads key head h // (H // Hk). blocks: int32
     [B, Hk, ceil(Sq / block_q), topk], as block_topk returns it: entries outside the sequence (-1) name nothing, an entry named twice counts
     twice. block_q, block_k: 64 or 128. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key, give
-    zeros and lse = -inf. scale: positive (2^-100 and more), default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq]). Differentiable once in q, k, v;
-    lse may carry a gradient too."""
+    zeros and lse = -inf. scale: positive (2^-100 and more), default D ** -0.5. Returns (out [B, Sq, H, D], lse fp32 [B, H, Sq]).
+    Differentiable once in q, k, v (reverse mode; a tensor with a tangent is refused); lse may carry a gradient too."""
     L.load_torch_ops()
     return torch.ops.sfast_xformers.block_sparse_attention(q, k, v, blocks, block_q, block_k, key_lengths, query_lengths, scale)
 

@@ -1,10 +1,11 @@
 """Attention over chosen blocks and rotary positions in the modes around them."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from sfast.hip import functional as F
 from sfast.hip import lib as L
-from test_video_attention_gpu import BF16, make, randn
+from test_video_attention_gpu import BF16, F32, grid, make, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,44 @@ def test_batch_invariant_mode_on_whole_query_blocks(H, D, monkeypatch):
     finally:
         monkeypatch.undo()
         assert lib.sfast_hip_init() == 0
+
+
+def test_there_are_no_derivatives_in_forward_mode():
+    """A tangent that is not carried on would count as zero."""
+    q, k, v, blocks = make((1, 100, 300, 2, 2, 64, 128, 64, 3, None, None), BF16)
+    pos = grid(1, 1, 300, 1, F32)
+    out, lse = F.block_sparse_attention(q, k, v, blocks)
+    calls = {
+        "rotary, query": lambda d: F.rotary_nd(d(k), None, pos, [64]),
+        "rotary, key": lambda d: F.rotary_nd(k, d(v), pos, [64]),
+        "rotary, positions": lambda d: F.rotary_nd(k, v, d(pos), [64]),
+        "means": lambda d: F.block_means(d(q), 64),
+        "query": lambda d: F.block_sparse_attention(d(q), k, v, blocks),
+        "key": lambda d: F.block_sparse_attention(q, d(k), v, blocks),
+        "value": lambda d: F.block_sparse_attention(q, k, d(v), blocks),
+        "backward, gradient": lambda d: F.block_sparse_attention_backward(d(out), None, q, k, v, blocks, out, lse),
+        "backward, gradient of lse": lambda d: F.block_sparse_attention_backward(out, d(lse), q, k, v, blocks, out, lse),
+        "backward, value": lambda d: F.block_sparse_attention_backward(out, None, q, k, d(v), blocks, out, lse),
+    }
+    for name, call in calls.items():
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+            call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+            raise AssertionError(name)
+        call(lambda t: t)   # the same call without a tangent
+    for f, x in ((lambda t: F.rotary_nd(t, None, pos, [64])[0], k), (lambda t: F.block_sparse_attention(t, k, v, blocks)[0], q)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+        with fwd.dual_level(), pytest.raises(RuntimeError):
+            f(fwd.make_dual(x.detach().requires_grad_(), torch.ones_like(x)))
+
+
+def test_gradients_that_were_called_for_are_not_differentiated_again():
+    """Leaves that want gradients go into the call as they are; only differentiating its results is refused."""
+    q, k, v, blocks = make((1, 100, 300, 2, 2, 64, 128, 64, 3, None, None), BF16)
+    out, lse = F.block_sparse_attention(q, k, v, blocks)
+    want = F.block_sparse_attention_backward(out, None, q, k, v, blocks, out, lse)
+    q.requires_grad_()
+    got = F.block_sparse_attention_backward(out, None, q, k, v, blocks, out, lse)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        got[1].sum().backward()
