@@ -1,11 +1,14 @@
-"""Attention over chosen blocks and rotary positions in the modes around them."""
+"""Attention over chosen blocks and rotary positions in the modes around them, and what a turn leaves alone."""
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+import video_attention_ref as R
 from sfast.hip import functional as F
 from sfast.hip import lib as L
-from test_video_attention_gpu import BF16, F32, grid, make, randn
+from test_video_attention_gpu import BF16, F16, F32, grid, make, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +76,24 @@ def test_gradients_that_were_called_for_are_not_differentiated_again():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(RuntimeError, match="second derivative"):
         got[1].sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D, sections", [(64, [16, 24]), (80, [30, 20]), (256, [128, 64]), (10, [2, 4])])
+def test_elements_behind_the_sections_are_copied_bit_by_bit(D, sections, interleaved, dtype):
+    """Infinities, NaN and negative zeros among them: a neighbour is not touched by them."""
+    used = sum(sections)
+    x = randn((2, 12, 3, D), dtype, 1)
+    tail = x[..., used:]
+    gen = torch.Generator().manual_seed(3)
+    odd = torch.tensor([math.inf, -math.inf, math.nan, -0.0, 0.0], dtype=dtype)
+    pick = torch.randint(0, 10, tail.shape, generator=gen)
+    tail.copy_(torch.where(pick < 5, odd[pick.clamp(max=4)], tail.cpu()))
+    assert not torch.isfinite(x[..., used:]).all()
+    bits = torch.int32 if dtype == F32 else torch.int16
+    pos = grid(1, 3, 4, 2, F32, 3, 0.7)
+    want, bound = R.rope(x[..., :used], pos, sections, 10000.0, interleaved)
+    for a in F.rotary_nd(x, x, pos, sections, interleaved=interleaved):
+        assert torch.equal(a[..., used:].contiguous().view(bits), x[..., used:].contiguous().view(bits))
+        R.check("turned", a[..., :used], want, bound)
