@@ -367,7 +367,7 @@ typedef struct {
     int32_t dtype;
     int32_t B, H, Sq, Skv, D;
     int64_t qs[3], ks[3], vs[3], os[3];
-    float scale; /* 2^-100 and more, finite */
+    float scale;
     int32_t variant;
 } sfast_attn_params;
 
@@ -576,7 +576,7 @@ typedef struct {
     int32_t dtype; /* f16 / bf16 */
     int32_t B, H, Hk, Sq, Sk, D, block_q, block_k, topk;
     int64_t qs[3], ks[3], vs[3], os[3];
-    float scale;
+    float scale; /* 2^-100 and more, finite */
     /* gradients only */
     int64_t dos[3], dqs[3], dks[3], dvs[3];
 } sfast_block_attn_params;
