@@ -9,6 +9,7 @@ generic HIP kernel inside the library instead).
 import ctypes as C
 import os
 import threading
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "_lib", "libsfast_hip.so")
@@ -311,7 +312,6 @@ def load():
         if lib.sfast_hip_abi_version() != ABI_VERSION:
             raise SfastHipError("libsfast_hip.so ABI version mismatch; rebuild")
         _lib = lib
-    load_torch_ops()
     return _lib
 
 
@@ -319,19 +319,29 @@ _torch_ops = False
 
 
 def load_torch_ops(required=True):
-    """Register the native operators (once). `required`: raise if they are not built, as load() does for the kernel library."""
+    """Register the native operators (once); True if they are there. `required`: raise if they are not, as load() does for the kernel library.
+    Otherwise (at import) a file that is not there is passed over, and one that does not load -- built for another torch, say -- is a warning:
+    nothing else needs it."""
     global _torch_ops
     if _torch_ops:
         return True
     with _lock:
-        if not _torch_ops:
-            if not os.path.exists(TORCH_OPS_PATH):
-                if required:
-                    raise SfastHipError(f"{TORCH_OPS_PATH} not found: build it with `python stable-fast_amd/build.py`. The native operators have no fallback.")
-                return False
-            import torch
+        if _torch_ops:
+            return True
+        if not os.path.exists(TORCH_OPS_PATH):
+            if required:
+                raise SfastHipError(f"{TORCH_OPS_PATH} not found: build it with `python stable-fast_amd/build.py`. The native operators have no fallback.")
+            return False
+        import torch
+        try:
             torch.ops.load_library(TORCH_OPS_PATH)
-            _torch_ops = True
+        except (OSError, RuntimeError) as e:
+            text = f"{TORCH_OPS_PATH} does not load ({e}): rebuild it with `python stable-fast_amd/build.py`. The native operators have no fallback."
+            if required:
+                raise SfastHipError(text) from e
+            warnings.warn(text, RuntimeWarning, stacklevel=2)
+            return False
+        _torch_ops = True
     return True
 
 
