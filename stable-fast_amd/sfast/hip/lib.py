@@ -325,24 +325,25 @@ def load_torch_ops(required=True):
     global _torch_ops
     if _torch_ops:
         return True
-    with _lock:
-        if _torch_ops:
-            return True
-        if not os.path.exists(TORCH_OPS_PATH):
-            if required:
-                raise SfastHipError(f"{TORCH_OPS_PATH} not found: build it with `python stable-fast_amd/build.py`. The native operators have no fallback.")
-            return False
-        import torch
-        try:
-            torch.ops.load_library(TORCH_OPS_PATH)
-        except (OSError, RuntimeError) as e:
-            text = f"{TORCH_OPS_PATH} does not load ({e}): rebuild it with `python stable-fast_amd/build.py`. The native operators have no fallback."
-            if required:
-                raise SfastHipError(text) from e
+    try:
+        if LIB_PATH == PROBES_LIB_PATH:
+            load()   # first: the native operators then call the probe build too (build.py gives it the product library's name)
+        with _lock:
+            if not _torch_ops:
+                if not os.path.exists(TORCH_OPS_PATH):
+                    raise SfastHipError(f"{TORCH_OPS_PATH} not found: build it with `python stable-fast_amd/build.py`. The native operators have no fallback.")
+                import torch
+                torch.ops.load_library(TORCH_OPS_PATH)
+                _torch_ops = True
+        return True
+    except (SfastHipError, OSError, RuntimeError) as e:
+        text = str(e) if isinstance(e, SfastHipError) else (f"{TORCH_OPS_PATH} does not load ({e}): rebuild it with `python stable-fast_amd/build.py`. "
+                                                            "The native operators have no fallback.")
+        if required:
+            raise SfastHipError(text) from e
+        if os.path.exists(TORCH_OPS_PATH) and os.path.exists(LIB_PATH):   # (before the first build there is nothing to warn of)
             warnings.warn(text, RuntimeWarning, stacklevel=2)
-            return False
-        _torch_ops = True
-    return True
+        return False
 
 
 _probes_lib = None

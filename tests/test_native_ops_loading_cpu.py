@@ -48,3 +48,22 @@ exists = os.path.exists
 os.path.exists = lambda p: exists(p) and not str(p).endswith("libsfast_torch.so")
 """ + USE)
     assert "libsfast_torch" not in r.stderr
+
+
+def test_the_probe_build_serves_the_native_operators_too(built_lib, built_probe_lib):
+    """SFAST_HIP_PROBES=1: one kernel library in the process, with one state, whichever operator is called."""
+    r = python("""
+import sfast
+from sfast.hip import lib as L
+assert L.load().sfast_hip_has_probes() and L.load_torch_ops()
+print(*sorted({line.split()[-1].rsplit("/", 1)[1] for line in open("/proc/self/maps") if "libsfast_" in line}))
+""", SFAST_HIP_PROBES="1")
+    assert r.stdout.split() == ["libsfast_hip_probes.so", "libsfast_torch.so"]
+    r = python("""
+import sfast
+from sfast.hip import lib as L
+assert not L.load().sfast_hip_has_probes() and L.load_torch_ops()
+assert L.load_probes().sfast_hip_has_probes() and not L.load().sfast_hip_has_probes()
+print(*sorted({line.split()[-1].rsplit("/", 1)[1] for line in open("/proc/self/maps") if "libsfast_" in line}))
+""")
+    assert r.stdout.split() == ["libsfast_hip.so", "libsfast_hip_probes.so", "libsfast_torch.so"]
