@@ -571,7 +571,8 @@ int sfast_hip_block_topk(const float *qm, const float *km, const int32_t *key_le
  * nothing, an entry named twice counts twice. Keys from key_lengths[b] on do not exist; rows from query_lengths[b] on, and rows without a key,
  * give zeros and lse = -inf. Lengths are clipped to [0, S]; NULL: full. q: [B, Sq, H, D], k / v: [B, Sk, Hk, D] (head h reads key head
  * h / (H / Hk)); strides (b, s, h) in elements, multiples of 8, head-dim stride 1, rows D to 2^23 elements apart, 16-byte aligned bases;
- * D % 8 == 0, D <= 128. out_rest (or NULL; laid out as out) receives what the rounding of out left behind, itself rounded to the type. */
+ * D % 8 == 0, D <= 128. The workspace holds fp32 partial results where lists are cut: where query blocks are few, and always from 1024 entries
+ * on. out_rest (or NULL; laid out as out) receives what the rounding of out left behind, itself rounded to the type. */
 typedef struct {
     int32_t dtype; /* f16 / bf16 */
     int32_t B, H, Hk, Sq, Sk, D, block_q, block_k, topk;
@@ -587,7 +588,8 @@ int sfast_hip_block_attention(const void *q, const void *k, const void *v, const
 /* Gradients of the call above from its out, lse and out_rest (or NULL: rowsum(dout * out) then keeps the error of out's rounding, which shows
  * in rows that attend to few keys), the gradient dout of out and (or NULL) dlse of lse [B, H, Sq] fp32. All of dq, dk, dv is
  * written (zeros where nothing reaches). Sums run in a fixed order: the same call gives the same bits. With delta = rowsum(dout * out) - dlse:
- * bf16 takes gradients of any magnitude; f16 gives NaN where |lse / scale| or |delta| reaches 2^31 and holds delta in steps of 2^-28. */
+ * bf16 takes gradients of any magnitude. The workspace holds 4 bytes for every pair of a key block and a query block of a key head (24 heads of
+ * a million tokens: 12.9 GB). f16 gives NaN where |lse / scale| or |delta| reaches 2^31 and holds delta in steps of 2^-28. */
 size_t sfast_hip_block_attention_backward_workspace_bytes(const sfast_block_attn_params *p);
 int sfast_hip_block_attention_backward(const void *q, const void *k, const void *v, const int32_t *blocks, const int32_t *key_lengths,
                                        const int32_t *query_lengths, const void *out, const void *out_rest, const float *lse,

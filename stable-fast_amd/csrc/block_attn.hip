@@ -11,8 +11,8 @@
 //
 // Measured, bf16: 32760 x 24 rows of 128 against 64 blocks of 64 each 1.64 ms, 1005 TFLOP/s (a library's matrix product of 8192^3: 1406);
 // 14400 x 20 rows of 64 against 32 blocks 176 us, 858 TFLOP/s. No single part bounds the first: without the exponentials (1540 us), the loads,
-// the LDS reads, or either product (1320 - 1360 each) it is faster by less than that part alone takes; the matrix pipe is busy half the time,
-// the VALU the other half. With heads of 64 the VALU has the more to do (32 exponentials at 16 cycles, 32 fused products and 32 additions a tile
+// the LDS reads, or either product (1320 - 1360 each) it is faster by less than that part alone takes; by the counters (8192 x 24 rows of 128) the
+// matrix pipe is busy 48 % of the time and the VALU 38 %, for heads of 64 38 % and 60 %. With heads of 64 the VALU has the more to do (32 exponentials at 16 cycles, 32 fused products and 32 additions a tile
 // of 64 keys and wave, 960 cycles against 512 of products). 4 x 8 rows of a token (32 heads) against 64 blocks of a long cache: 16 + 4 us, 50 MB.
 // Tried and left: a tile's products under the next tile's softmax, raised wave priorities, the reference as the products' start
 // (the compiler copies the registers), four waves a SIMD for heads of 64 (177 -> 195 us).
@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(NW * KW * 64, 2) block_attn_fwd_kernel(const B
                 for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
         }
         const float ref = m == -INFINITY ? 0.f : m;  // a row whose scores are all -inf keeps the sum 0
+        // the sum takes the probabilities in fp32, the product with V takes them rounded to the type: half a step each, so that out is off by 1.1
+        // times (5 keys) to 1.4 times (many) what its own rounding alone would give
         vec8 p[2 * KBN];
 #pragma unroll
         for (int kb = 0; kb < KBN; ++kb)
@@ -396,7 +398,7 @@ template <typename T, int DP> int launch(const BlockAttnArgs &a, const Plan &pl,
     int rc = check_launch("block_attention");
     if (rc || pl.nsplit == 1) return rc;
     const int per = pl.pack ? a.Sq * a.G : a.bq;
-    const int rows = (int)(pl.units * per);  // (a split call has few units)
+    const int rows = (int)(pl.units * per);  // (the entry point holds units * 128 rows of a split call below 2^26)
     const dim3 jgrid((unsigned)ceil_div(rows, 4));
     if (pl.pack)
         hipLaunchKernelGGL((block_attn_join_kernel<T, true>), jgrid, dim3(256), 0, st, a, pl.nw * 32, rows);

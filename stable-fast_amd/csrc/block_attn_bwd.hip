@@ -118,11 +118,11 @@ __global__ void __launch_bounds__(256) block_attn_count_kernel(const BlockAttnAr
     if (j >= 0 && (int64_t)j * a.bk < klen) atomicAdd(a.cnt + ((int64_t)pair * a.nK + j) * a.nQ + qb, 1);
 }
 
-// Probabilities and dS are rounded to the type for the products that sum them, which about doubles the square of a gradient's error (1.42 times
-// one rounding's). With FINE the part that this rounding cuts off takes part as well, in products of its own: the gradient keeps its last
-// rounding alone. For calls of one query or one key block: there a single probability can weigh most (errors up to 1.9 times one rounding's
-// without it), and the time is that of a chain of small steps (100 x 16 query rows of 64 against 16 blocks of 64: 43.5 -> 47 us; the whole
-// grids would pay a third).
+// Probabilities and dS are rounded to the type for the products that sum them, which doubles the square of a gradient's error: 1.42 times one
+// rounding's, measured alike for lists of 1 to 30 blocks and for 5 keys. With FINE the part that this rounding cuts off takes part as well, in
+// products of its own: the gradient keeps its last rounding alone. The rule is what that costs. Calls of one query or one key block have it:
+// their time is that of a chain of small steps (100 x 16 query rows of 64 against 16 blocks of 64: 43.5 -> 47 us). Whole grids would pay a third.
+// f16: a dS below 2^-14 loses digits and below 2^-25 is 0 (the cut-off part is smaller still), so small losses want a scale, as for any f16 gradient.
 template <typename T, bool FINE> struct BbRounded {
     typename Elem<T>::vec8 v, rest;
     __device__ __forceinline__ void set(int i, float x) {

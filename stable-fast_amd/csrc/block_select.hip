@@ -1,7 +1,8 @@
 // Which key blocks a query block attends to: block means (sfast_hip_block_means) and the choice by their products (sfast_hip_block_topk).
 //
-// Sums and products run in 64 bits: a choice stands on which of two scores is larger, and in 64 bits the order of the additions does not
-// decide that (products of two fp32 means are exact, sums lose 2^-53).
+// Sums and products run in 64 bits: a choice stands on which of two scores is larger. Products of two fp32 means are exact then, and sums lose
+// 2^-53 a step, so the order of the additions (which differs between the score kernels below) can decide only between scores that agree to about
+// 2^-53 of their terms' magnitudes. Within a call all blocks' scores are summed in one order: equal means give equal scores.
 #include "common.h"
 #include <math.h>
 
@@ -12,7 +13,7 @@ namespace {
 // ---- block means ------------------------------------------------------------------------------------------------------------------------
 // Bound by reading x. A workgroup owns one block and 32 runs of V elements (512 bytes of a contiguous token); 8 groups of threads share its
 // rows, each thread keeps several 16-byte loads in flight, and the groups' sums are added in LDS in a fixed order.
-// (57600 x 10 rows of 64 in bf16: 13.4 us, 5.6 TB/s; 4 x 8191 x 8 rows of 128, ragged: 9.7 us, of which 2 are the launch.)
+// (57600 x 10 rows of 64 in f16: 13.4 us, 5.6 TB/s; 4 x 8191 x 8 rows of 128, ragged: 9.7 us, of which 2 are the launch.)
 struct MeansArgs {
     const void *x;
     const int32_t *lengths;

@@ -285,10 +285,6 @@ _def("linear_relu(Tensor input, Tensor weight, Tensor? bias=None) -> Tensor", li
 _def("linear_gelu(Tensor input, Tensor weight, Tensor? bias=None) -> Tensor", linear_gelu)
 
 
-# ---- rotary positions with several axes (no counterpart in the reference): `sfast::rotary_embedding_nd` is a native operator, registered by
-# csrc/torch/video_attention.cpp when the package is imported; hip.functional.rotary_nd says what it does -------------------------------------
-
-
 # ---- int8 dynamic linear (reference csrc/operators/cutlass/cutlass_qlinear.cc:10-89) ---------------------------------------------
 # The reference does not add an operator of its own shape here: it OVERRIDES `quantized::linear_dynamic(X, W_prepack, reduce_range)`
 # for the CUDA / QuantizedCUDA dispatch keys (cutlass_qlinear.cc:73-81), so that `torch.quantization.quantize_dynamic(unet)` modules
