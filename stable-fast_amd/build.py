@@ -123,8 +123,8 @@ def build(force=False, jobs=None, verbose=True, probes=False):
                 if verbose:
                     print(f"[sfast build] compiled {os.path.basename(done)}", flush=True)
     stamp = os.path.join(OBJ_DIR, "link_probes.stamp" if probes else "link.stamp")
-    # the probe build answers to the product library's name: where it was loaded first, libsfast_torch.so's calls go to it as well
-    link_flags = ["-Wl,-soname,libsfast_hip.so"] if probes else []
+    # both builds carry one name: libsfast_torch.so's calls go to whichever was loaded first
+    link_flags = ["-Wl,-soname,libsfast_hip.so"]
     link_tag = _digest(objs, ["link"] + link_flags)
     old = open(stamp).read() if os.path.exists(stamp) else ""
     if force or tasks or not os.path.exists(lib_path) or old != link_tag:
