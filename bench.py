@@ -976,6 +976,17 @@ def bench_svd(args, dev, rank, world, use_dist):
     print(json.dumps(out), flush=True)
 
 
+def contract_line(out, most=6000):
+    """(the line for stdout, what was moved out of it). A reader that keeps the last few KB of the output has to find the whole line in them:
+    beyond `most` characters the variants' own reports (their values stay in variants_summary) and the kernel families leave it."""
+    details = {}
+    for k in ("variants", "kernel_families"):
+        if k in out and len(json.dumps(out)) > most:
+            details[k] = out[k]
+            out = {n: v for n, v in out.items() if n != k}
+    return out, details
+
+
 def torchrun_argv(n, argv, port=None):
     """Command that re-launches this script as `n` ranks of one node (what the driver does itself for N > 1)."""
     if port is None:
@@ -1170,7 +1181,7 @@ def main():
             out["end_to_end"] = e2e
             if "ms_per_image_end_to_end" in e2e:
                 out["ms_per_image_end_to_end"] = e2e["ms_per_image_end_to_end"]
-        # headline values of the variant legs at the FRONT of the line: the driver keeps a truncated tail of long lines
+        # headline values of the variant legs at the front of the line
         v = out.get("variants") if isinstance(out.get("variants"), dict) else {}
         summ = {k: {"value": v[k]["value"], "unit": v[k].get("unit"), "ms_per_step": v[k].get("ms_per_step"),
                     "workload": (v[k].get("config") or {}).get("workload", k)}
@@ -1179,6 +1190,9 @@ def main():
             head = {k: out[k] for k in ("metric", "value", "unit") if k in out}
             head["variants_summary"] = summ
             out = {**head, **{k: val for k, val in out.items() if k not in head}}
+        out, details = contract_line(out)
+        if details:
+            print(json.dumps({"details": details}), file=sys.stderr, flush=True)
         print(json.dumps(out), flush=True)
     if use_dist:
         dist.destroy_process_group()
